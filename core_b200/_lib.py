@@ -70,11 +70,26 @@ class CoreCompressArgs(ctypes.Structure):
     ]
 
 
+class CoreKvq(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("k_meta", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("v_meta", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("bits", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
 _S = ctypes.c_size_t
 _D = ctypes.POINTER(CoreDims)
+_Q = ctypes.POINTER(CoreKvq)
 
 # name -> (restype, argtypes); mirrors include/core_b200.h
 SIGNATURES = {
@@ -121,6 +136,11 @@ SIGNATURES = {
     "core_rope_queries": (ctypes.c_int, [_I, _I, _I, _I, _I, _P, ctypes.c_int64, _P, _P, _F, _P,
                                          _P, _I, _P, _P]),
     "core_attention_prefill": (ctypes.c_int, [_D, _P, _P, _P, _P, _P, _P, _P, _P, _F, _P]),
+    "core_kvq_quantize": (ctypes.c_int, [_Q, _I, _P, _P, _P, _P, _I, _I, _P, _P, _I, _P, _P]),
+    "core_kvq_dequantize": (ctypes.c_int, [_Q, _I, _I, _P, _P, _I, _P, _P, _P]),
+    "core_kvq_attention_workspace_bytes": (_S, [_Q, _I, _I, _I]),
+    "core_kvq_attention": (ctypes.c_int, [_Q, _I, _I, _I, _P, _P, _P, _I, _P, ctypes.c_int64, _I,
+                                          _F, _P, _P, _P, _S, _P]),
     "core_compress_layer_workspace_bytes": (_S, [_D, _I, _I]),
     "core_compress_layer": (ctypes.c_int, [_D, _P, _P, _P, _P, _P, _P,
                                            ctypes.POINTER(CoreLayerWeights),

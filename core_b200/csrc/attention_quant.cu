@@ -1,0 +1,796 @@
+// Attention over the quantised KV cache (4 or 8 bits), for few query rows a KV
+// head: single tokens, short runs of proposed tokens.
+//
+//   S = scale q (n s + z)^T,  out = softmax(S) (n s + z),  LSE = log sum exp S
+//
+// What bounds it: the packed cache is read once, 16 bits + 4 (128 / group)
+// bytes a row of K or V; beside that, every code has to be turned into a matrix
+// operand, and at 6.5 TB/s an SM has about two instructions a code to do it.
+//
+//  * The codes are the A operand (16 tokens, or 16 channels, a tile) and the
+//    query rows the 8 columns of B, so that a GQA group of up to 8 rows wastes
+//    little; S^T comes out with a token per row and goes back in as the B
+//    operand of P V through movmatrix, without leaving the registers.
+//  * K's codes enter as exact integers: a nibble masked out of its word is the
+//    f16 subnormal n 2^-24 (or 16 n 2^-24; q then carries the 1/16).  A group's
+//    products are multiplied by its scale in f32, and the zeros come in through
+//    one more product, z times the row's sum of q over the group (as two f16
+//    terms), so that S has no rounding but f32's.  q is scaled by a power of two
+//    to f16's range per row; bf16 and f16 queries stay exact.
+//  * V's codes are spread over tokens in the scale that multiplies them, so
+//    they become f16 values n s + z (one rounding, 2^-12) in registers.
+//  * A warp owns 32-token tiles (every fourth of its CTA's) with its own ring of
+//    bulk copies, running maxima and sums: nothing waits for another warp until
+//    the CTA's four results are joined.  The maximum is raised only when a score
+//    passes it by 2^8.
+//  * A sequence is cut over CTAs when there are few (batch row, KV head) pairs;
+//    a second kernel joins the parts.
+#include <cuda_bf16.h>
+
+#include <climits>
+#include <cmath>
+
+#include "common.cuh"
+#include "host_util.h"
+#include "kvq_common.cuh"
+
+namespace core {
+namespace kvq {
+
+constexpr int kWarps = 4;
+constexpr int kAttnThreads = kWarps * 32;
+constexpr int kTok = 32;  // tokens of a warp's tile
+constexpr float kRaise = 8.0f;  // P <= 2^8 before the maximum is raised
+
+struct AttnParams {
+  const uint8_t* kc;
+  const uint32_t* km;
+  const uint8_t* vc;
+  const uint32_t* vm;
+  const void* q;
+  long long qb, qh, ql;  // element strides of (B, Hq, Lq)
+  const int* lengths;    // (B), or null: max_len for all
+  const uint8_t* mask;   // (B, mask_stride), 0: hidden; or null
+  long long mask_stride;
+  int B, Hkv, G, Lq, cap, max_len;
+  int n_rt, n_split;  // row tiles a KV head, parts of a sequence
+  int causal, f16;
+  float scale_log2;
+  void* out;    // (B, Lq, Hq, d)
+  float* lse;   // (B, Hq, Lq), natural log
+  float* part_o;    // (B Hkv, row, split, d) f32 where n_split > 1
+  float* part_lse;  // (B Hkv, row, split), base 2
+  DeviceStatus* status;
+};
+
+template <int kBits, int kG>
+struct Stage {
+  static constexpr uint32_t kCodes = kTok * 16 * kBits, kMeta = kTok * 4 * kG;
+  static constexpr uint32_t kKc = 0, kVc = kCodes, kKm = 2 * kCodes, kVm = kKm + kMeta, kBytes = kVm + kMeta;
+  static constexpr int kCount = kBits == 4 ? 4 : 3;
+};
+
+// Tokens of one sequence that the kernel sees.
+__device__ __forceinline__ int sequence_length(const AttnParams& p, int b) {
+  int n = p.max_len;
+  if (p.lengths != nullptr) {
+    const int given = p.lengths[b];
+    if (given < 0 || given > p.max_len) {
+      if (threadIdx.x == 0) record_error(p.status, CORE_ERR_INVALID_ARG, 1421, b);
+      n = given < 0 ? 0 : p.max_len;
+    } else {
+      n = given;
+    }
+  }
+  return n;
+}
+
+// Last token (exclusive) that query row r of a KV head sees; rows past the end see none.
+__device__ __forceinline__ int row_limit(const AttnParams& p, int r, int len) {
+  const int i = r / p.G;
+  if (i >= p.Lq) return 0;
+  return p.causal ? max(len - p.Lq + i + 1, 0) : len;
+}
+
+// Warp tiles of a sequence and the ones of a part.
+__device__ __forceinline__ int tiles_per_split(int end, int n_split) {
+  const int tiles = (end + kTok - 1) / kTok;
+  return (tiles + n_split - 1) / n_split;
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ float low_half(uint32_t w) { return __low2float(as_half2(w)); }
+
+// Query rows [8 nt, 8 nt + 8) of a tile as B operands: lane (g, t) holds of row g
+// the channels 32 b + 8 t .. + 7, in pairs i = 0..3: reg 4 b + i.
+template <int kBits, int kG>
+__device__ __forceinline__ void load_queries(const AttnParams& p, int b, int kvh, int row, int t, uint32_t (&qf)[16],
+                                             uint32_t& qsum, float& row_scale) {
+  const int i = row / p.G;
+  float x[32];
+  float mx = 0.f;
+  const bool live = i < p.Lq;
+  const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.qb +
+                        (long long)(kvh * p.G + (live ? row - i * p.G : 0)) * p.qh + (long long)(live ? i : 0) * p.ql;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (live) u = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * t);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float2 f;
+      if (p.f16)
+        f = __half22float2(as_half2(w[j]));
+      else
+        f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+      x[8 * c + 2 * j] = f.x;
+      x[8 * c + 2 * j + 1] = f.y;
+      mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
+    }
+  }
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+  // power of two that brings the row's largest element into [2^7, 2^8); the two
+  // factors keep it within f32 for any exponent
+  const int e = (int)((__float_as_uint(mx) >> 23) & 255u) - 127;
+  const int sh = mx > 0.f && e < 128 ? 7 - e : 0;
+  const int sh1 = sh / 2, sh2 = sh - sh1;
+  const float f1 = __uint_as_float((uint32_t)(127 + sh1) << 23), f2 = __uint_as_float((uint32_t)(127 + sh2) << 23);
+  float part[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    part[c] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = __floats2half2_rn(x[8 * c + 2 * j] * f1 * f2, x[8 * c + 2 * j + 1] * f1 * f2);
+      const float2 r = __half22float2(h);
+      part[c] += r.x + r.y;
+      // 4 bits: odd pairs meet 16 n
+      qf[4 * c + j] = as_u32(kBits == 4 && (j & 1) ? __hmul2(h, __floats2half2_rn(0.0625f, 0.0625f)) : h);
+    }
+    part[c] += __shfl_xor_sync(0xffffffffu, part[c], 1);
+    part[c] += __shfl_xor_sync(0xffffffffu, part[c], 2);
+  }
+  // sum of q over group t (t < kG), as two f16 terms
+  float s;
+  if (kG == 4)
+    s = t == 0 ? part[0] : t == 1 ? part[1] : t == 2 ? part[2] : part[3];
+  else if (kG == 2)
+    s = t == 0 ? part[0] + part[1] : t == 1 ? part[2] + part[3] : 0.f;
+  else
+    s = t == 0 ? (part[0] + part[1]) + (part[2] + part[3]) : 0.f;
+  const __half hi = __float2half_rn(s);
+  qsum = as_u32(__halves2half2(hi, __float2half_rn(s - __half2float(hi))));
+  // S = raw * row_scale with raw in units of 2^-24 2^sh
+  row_scale = p.scale_log2 * 16777216.f;
+  row_scale = row_scale * __uint_as_float((uint32_t)(127 - sh1) << 23) * __uint_as_float((uint32_t)(127 - sh2) << 23);
+}
+
+template <int kBits, int kG, int kNT>
+__global__ void __launch_bounds__(kAttnThreads) attn_few_kernel(const AttnParams p) {
+  using St = Stage<kBits, kG>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kWarps * St::kCount];
+  __shared__ int abort_storage;
+  __shared__ float sm_m[kWarps][8 * kNT], sm_l[kWarps][8 * kNT];
+  volatile int* abort_flag = &abort_storage;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  unsigned u = blockIdx.x;
+  const int rt = (int)(u % (unsigned)p.n_rt);
+  u /= (unsigned)p.n_rt;
+  const int split = (int)(u % (unsigned)p.n_split);
+  const int bh = (int)(u / (unsigned)p.n_split);
+  const int b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  const int row0 = rt * 8 * kNT;
+  const int rows = p.G * p.Lq;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWarps * St::kCount; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    abort_storage = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+
+  const int len = sequence_length(p, b);
+  const int last_row = min(row0 + 8 * kNT, rows) - 1;
+  const int end = row_limit(p, last_row, len);  // no row of the tile sees a token from here on
+  const int first_end = row_limit(p, row0, len);  // every row sees the tokens before this
+  const int per = tiles_per_split(end, p.n_split);
+  const int tile0 = split * per, tile1 = min(tile0 + per, (end + kTok - 1) / kTok);
+  if (p.n_split > 1 && tile0 >= tile1 && split > 0) return;  // the join does not read this part
+
+  const long long base = (long long)bh * p.cap;
+  const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (St::kCount * St::kBytes);
+  const uint32_t my_bars = smem_u32(&bars[warp * St::kCount]);
+  const int n_mine = tile1 - tile0 > warp ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;
+  auto issue = [&](int it) {
+    const int s = it % St::kCount;
+    const long long row = base + (long long)(tile0 + warp + it * kWarps) * kTok;
+    const uint32_t bar = my_bars + 8u * s, dst = ring + s * St::kBytes;
+    mbar_arrive_expect_tx(bar, St::kBytes);
+    bulk_load(dst + St::kKc, p.kc + row * (16 * kBits), St::kCodes, bar);
+    bulk_load(dst + St::kKm, p.km + row * kG, St::kMeta, bar);
+    bulk_load(dst + St::kVc, p.vc + row * (16 * kBits), St::kCodes, bar);
+    bulk_load(dst + St::kVm, p.vm + row * kG, St::kMeta, bar);
+  };
+  if (lane == 0)
+    for (int it = 0; it < St::kCount && it < n_mine; ++it) issue(it);
+
+  uint32_t qf[kNT][16], qsum[kNT];
+  float rs[kNT][2];
+  int lim[kNT][2];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    float r;
+    load_queries<kBits, kG>(p, b, kvh, row0 + 8 * n + g, t, qf[n], qsum[n], r);
+    rs[n][0] = __shfl_sync(0xffffffffu, r, 8 * t);      // row 2 t of the eight
+    rs[n][1] = __shfl_sync(0xffffffffu, r, 8 * t + 4);  // row 2 t + 1
+    lim[n][0] = row_limit(p, row0 + 8 * n + 2 * t, len);
+    lim[n][1] = row_limit(p, row0 + 8 * n + 2 * t + 1, len);
+  }
+
+  float o[8][kNT][4];
+  float m_used[kNT][2], l[kNT][2];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    m_used[n][0] = m_used[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
+  }
+
+  // Row r of a 16-token tile holds token pi(r): pi(2 i) = i, pi(2 i + 1) = 4 +
+  // (i ^ 1), pi(r + 8) = pi(r) + 8: lanes that read K or V together then never
+  // meet in a bank.
+  const int pig = (g & 1) ? 4 + ((g >> 1) ^ 1) : g >> 1;  // token of K row g
+  const int va = t, vb = 4 + (t ^ 1);                     // tokens of V columns 2 t and 2 t + 1
+  const int vgrp = (g * kG) >> 3;                         // group of V channels 16 g ..
+
+  const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (long long)b * p.mask_stride;
+  bool ok = true;
+  for (int it = 0; it < n_mine; ++it) {
+    const int s = it % St::kCount;
+    const int tok0 = (tile0 + warp + it * kWarps) * kTok;
+    bool seen = tok0 + lane < end;
+    if (mask != nullptr && seen) seen = mask[tok0 + lane] != 0;
+    const uint32_t bits = __ballot_sync(0xffffffffu, seen);
+    ok = bounded_wait(my_bars + 8u * s, (uint32_t)(it / St::kCount) & 1u, abort_flag, p.status, 1422);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) {  // give up, but leave no copy of this warp's in flight
+      for (int k = it; k < it + St::kCount && k < n_mine; ++k) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(my_bars + 8u * (k % St::kCount), (uint32_t)(k / St::kCount) & 1u) &&
+               globaltimer_ns() - t0 < kWaitLimitNs) {
+        }
+      }
+      break;
+    }
+    const uint32_t st = ring + s * St::kBytes;
+
+    // ---- S^T: two tiles of 16 tokens, kNT tiles of 8 rows
+    float sc[2][kNT][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const uint32_t tk0 = 16 * mt + pig, tk1 = tk0 + 8;
+      uint32_t m0[kG], m1[kG];
+      const uint32_t ma = st + St::kKm;
+      if constexpr (kG == 4) {
+        const uint4 x = lds128(ma + tk0 * 16), y = lds128(ma + tk1 * 16);
+        m0[0] = x.x; m0[1] = x.y; m0[2] = x.z; m0[3] = x.w;
+        m1[0] = y.x; m1[1] = y.y; m1[2] = y.z; m1[3] = y.w;
+      } else if constexpr (kG == 2) {
+        const uint2 x = lds64(ma + tk0 * 8), y = lds64(ma + tk1 * 8);
+        m0[0] = x.x; m0[1] = x.y;
+        m1[0] = y.x; m1[1] = y.y;
+      } else {
+        m0[0] = lds32(ma + tk0 * 4);
+        m1[0] = lds32(ma + tk1 * 4);
+      }
+      // zeros: column 2 t, 2 t + 1 of the product both hold group t's
+      uint32_t z0 = 0, z1 = 0;
+      if constexpr (kG == 4) {
+        z0 = lds32(ma + tk0 * 16 + t * 4);
+        z1 = lds32(ma + tk1 * 16 + t * 4);
+      } else if constexpr (kG == 2) {
+        z0 = t == 0 ? m0[0] : t == 1 ? m0[1] : 0u;
+        z1 = t == 0 ? m1[0] : t == 1 ? m1[1] : 0u;
+      } else {
+        z0 = t == 0 ? m0[0] : 0u;
+        z1 = t == 0 ? m1[0] : 0u;
+      }
+      z0 = prmt(z0, z0, 0x3232);
+      z1 = prmt(z1, z1, 0x3232);
+      float zs[kNT][4];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        zs[n][0] = zs[n][1] = zs[n][2] = zs[n][3] = 0.f;
+        mma1688(zs[n], z0, z1, qsum[n]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[mt][n][e] = zs[n][e] * 5.9604644775390625e-8f;  // 2^-24
+      }
+      // codes: words of block b of 32 channels (8 bits: two words)
+      uint32_t w0[kBits], w1[kBits];
+#pragma unroll
+      for (int c = 0; c < kBits / 4; ++c) {
+        const uint32_t at0 = (64u * c + 16u * t) ^ key_swizzle<kBits>(tk0), at1 = (64u * c + 16u * t) ^ key_swizzle<kBits>(tk1);
+        const uint4 x = lds128(st + St::kKc + tk0 * (16 * kBits) + at0), y = lds128(st + St::kKc + tk1 * (16 * kBits) + at1);
+        w0[4 * c] = x.x; w0[4 * c + 1] = x.y; w0[4 * c + 2] = x.z; w0[4 * c + 3] = x.w;
+        w1[4 * c] = y.x; w1[4 * c + 1] = y.y; w1[4 * c + 2] = y.z; w1[4 * c + 3] = y.w;
+      }
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) {
+        float acc[kNT][4];
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+        for (int bb = 0; bb < 4 / kG; ++bb) {
+          const int blk = gr * (4 / kG) + bb;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // pairs 2 h and 2 h + 1: 16 channels of the quad
+            uint32_t a0, a1, a2, a3;
+            if constexpr (kBits == 4) {
+              const uint32_t x0 = h ? w0[blk] >> 8 : w0[blk], x1 = h ? w1[blk] >> 8 : w1[blk];
+              a0 = x0 & 0x000f000fu;
+              a1 = x1 & 0x000f000fu;
+              a2 = x0 & 0x00f000f0u;
+              a3 = x1 & 0x00f000f0u;
+            } else {
+              const uint32_t x0 = w0[2 * blk + h], x1 = w1[2 * blk + h];
+              a0 = x0 & 0x00ff00ffu;
+              a1 = x1 & 0x00ff00ffu;
+              a2 = (x0 >> 8) & 0x00ff00ffu;
+              a3 = (x1 >> 8) & 0x00ff00ffu;
+            }
+#pragma unroll
+            for (int n = 0; n < kNT; ++n)
+              mma16816(acc[n], a0, a1, a2, a3, qf[n][4 * blk + 2 * h], qf[n][4 * blk + 2 * h + 1]);
+          }
+        }
+        const float s0 = low_half(m0[gr]), s1 = low_half(m1[gr]);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          sc[mt][n][0] = fmaf(s0, acc[n][0], sc[mt][n][0]);
+          sc[mt][n][1] = fmaf(s0, acc[n][1], sc[mt][n][1]);
+          sc[mt][n][2] = fmaf(s1, acc[n][2], sc[mt][n][2]);
+          sc[mt][n][3] = fmaf(s1, acc[n][3], sc[mt][n][3]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[mt][n][e] *= rs[n][e & 1];
+    }
+    const bool full = bits == 0xffffffffu && tok0 + kTok <= first_end;
+    if (!full) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int n = 0; n < kNT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 16 * mt + pig + (e >> 1) * 8;
+            if (!((bits >> k) & 1u) || tok0 + k >= lim[n][e & 1]) sc[mt][n][e] = -INFINITY;
+          }
+    }
+
+    // ---- running maxima
+    bool raise = false;
+    float mx[kNT][2];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[n][h] = fmaxf(fmaxf(sc[0][n][h], sc[0][n][h + 2]), fmaxf(sc[1][n][h], sc[1][n][h + 2]));
+        raise |= mx[n][h] > m_used[n][h] + kRaise;
+      }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v = mx[n][h];
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          if (v > m_used[n][h] + kRaise) {
+            const float f = ex2_approx(m_used[n][h] - v);
+            m_used[n][h] = v;
+            l[n][h] *= f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              o[j][n][h] *= f;
+              o[j][n][h + 2] *= f;
+            }
+          }
+        }
+    }
+
+    // ---- P^T, and its transpose as the B operand
+    uint32_t pf[2][kNT][2];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      const float b0 = m_used[n][0] == -INFINITY ? 0.f : m_used[n][0];
+      const float b1 = m_used[n][1] == -INFINITY ? 0.f : m_used[n][1];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const float e0 = ex2_approx(sc[mt][n][0] - b0), e1 = ex2_approx(sc[mt][n][1] - b1);
+        const float e2 = ex2_approx(sc[mt][n][2] - b0), e3 = ex2_approx(sc[mt][n][3] - b1);
+        l[n][0] += e0 + e2;
+        l[n][1] += e1 + e3;
+        pf[mt][n][0] = movmatrix_trans(as_u32(__floats2half2_rn(e0, e1)));
+        pf[mt][n][1] = movmatrix_trans(as_u32(__floats2half2_rn(e2, e3)));
+      }
+    }
+
+    // ---- O^T += V^T P^T
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const uint32_t ta = 16 * mt + va, tb = 16 * mt + vb;
+      const uint32_t ma = st + St::kVm + vgrp * 4;
+      uint32_t xa = lds32(ma + ta * (4 * kG)), xb = lds32(ma + tb * (4 * kG));
+      uint32_t ya = lds32(ma + (ta + 8) * (4 * kG)), yb = lds32(ma + (tb + 8) * (4 * kG));
+      if (bits != 0xffffffffu) {  // hidden tokens: value 0, whatever their bytes hold
+        xa = (bits >> ta) & 1u ? xa : 0u;
+        xb = (bits >> tb) & 1u ? xb : 0u;
+        ya = (bits >> (ta + 8)) & 1u ? ya : 0u;
+        yb = (bits >> (tb + 8)) & 1u ? yb : 0u;
+      }
+      const __half2 sx = as_half2(prmt(xa, xb, 0x5410)), zx = as_half2(prmt(xa, xb, 0x7632));
+      const __half2 sy = as_half2(prmt(ya, yb, 0x5410)), zy = as_half2(prmt(ya, yb, 0x7632));
+      const uint32_t vs = st + St::kVc;
+      uint32_t wa[kBits / 2], wb[kBits / 2], ua[kBits / 2], ub[kBits / 2];
+      if constexpr (kBits == 4) {
+        const uint32_t at = (8u * g) ^ value_swizzle<4>(ta);  // alike for all four tokens
+        const uint2 r0 = lds64(vs + ta * 64 + at), r1 = lds64(vs + tb * 64 + at);
+        const uint2 r2 = lds64(vs + (ta + 8) * 64 + at), r3 = lds64(vs + (tb + 8) * 64 + at);
+        wa[0] = r0.x; wa[1] = r0.y; wb[0] = r1.x; wb[1] = r1.y;
+        ua[0] = r2.x; ua[1] = r2.y; ub[0] = r3.x; ub[1] = r3.y;
+      } else {
+        const uint32_t ata = (16u * g) ^ value_swizzle<8>(ta), atb = (16u * g) ^ value_swizzle<8>(tb);
+        const uint4 r0 = lds128(vs + ta * 128 + ata), r1 = lds128(vs + tb * 128 + atb);
+        const uint4 r2 = lds128(vs + (ta + 8) * 128 + ata), r3 = lds128(vs + (tb + 8) * 128 + atb);
+        wa[0] = r0.x; wa[1] = r0.y; wa[2] = r0.z; wa[3] = r0.w;
+        wb[0] = r1.x; wb[1] = r1.y; wb[2] = r1.z; wb[3] = r1.w;
+        ua[0] = r2.x; ua[1] = r2.y; ua[2] = r2.z; ua[3] = r2.w;
+        ub[0] = r3.x; ub[1] = r3.y; ub[2] = r3.z; ub[3] = r3.w;
+      }
+#pragma unroll
+      for (int w = 0; w < kBits / 2; ++w) {
+        // even channels of the word for both tokens, and odd ones
+        const uint32_t ex = prmt(wa[w], wb[w], 0x5410), ox = prmt(wa[w], wb[w], 0x7632);
+        const uint32_t ey = prmt(ua[w], ub[w], 0x5410), oy = prmt(ua[w], ub[w], 0x7632);
+#pragma unroll
+        for (int i = 0; i < 16 / kBits; ++i) {
+          const uint32_t a0 = as_u32(__hfma2(code_pair<kBits>(ex, i), sx, zx));
+          const uint32_t a1 = as_u32(__hfma2(code_pair<kBits>(ox, i), sx, zx));
+          const uint32_t a2 = as_u32(__hfma2(code_pair<kBits>(ey, i), sy, zy));
+          const uint32_t a3 = as_u32(__hfma2(code_pair<kBits>(oy, i), sy, zy));
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+            mma16816(o[w * (16 / kBits) + i][n], a0, a1, a2, a3, pf[mt][n][0], pf[mt][n][1]);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0 && it + St::kCount < n_mine) issue(it + St::kCount);
+  }
+
+  // ---- join the warps: maxima and sums, then each channel's weighted sum
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v = l[n][h];
+      v += __shfl_xor_sync(0xffffffffu, v, 4);
+      v += __shfl_xor_sync(0xffffffffu, v, 8);
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+      if (g == 0) {
+        sm_m[warp][8 * n + 2 * t + h] = m_used[n][h];
+        sm_l[warp][8 * n + 2 * t + h] = v;
+      }
+    }
+  __syncthreads();  // also: every warp's ring is idle
+  if (*abort_flag) return;
+  float* so = reinterpret_cast<float*>(smem);  // [warp][row][128]
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* dst = so + ((warp * 8 * kNT) + 8 * n + 2 * t + h) * kD + 16 * g;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        // m-tile j: channels 2 j (row g) and 2 j + 1 (row g + 8) of the sixteen
+        *reinterpret_cast<float4*>(dst + 2 * j) =
+            make_float4(o[j][n][h], o[j][n][h + 2], o[j + 1][n][h], o[j + 1][n][h + 2]);
+      }
+    }
+  __syncthreads();
+  const int c = threadIdx.x;
+  for (int r = 0; r < 8 * kNT && row0 + r < rows; ++r) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm_m[w][r]);
+    const float mb = m == -INFINITY ? 0.f : m;
+    float lt = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2_approx(sm_m[w][r] - mb);
+      lt += f * sm_l[w][r];
+      acc += f * so[(w * 8 * kNT + r) * kD + c];
+    }
+    // a row that saw no token: output 0, LSE -inf.  (NaN scores leave lt NaN.)
+    const float val = lt == 0.f ? 0.f : acc / lt;
+    const float lse2 = lt == 0.f ? -INFINITY : m + log2f(lt);
+    const int i = (row0 + r) / p.G, hq = kvh * p.G + (row0 + r) - i * p.G;
+    if (p.n_split > 1) {
+      const long long at = ((long long)bh * rows + row0 + r) * p.n_split + split;
+      p.part_o[at * kD + c] = val;
+      if (c == 0) p.part_lse[at] = lse2;
+    } else {
+      const int Hq = p.Hkv * p.G;
+      const long long at = (((long long)b * p.Lq + i) * Hq + hq) * kD + c;
+      if (p.f16)
+        static_cast<__half*>(p.out)[at] = __float2half_rn(val);
+      else
+        static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(val);
+      if (c == 0) p.lse[((long long)b * Hq + hq) * p.Lq + i] = lse2 * 0.69314718055994531f;
+    }
+  }
+}
+
+// Joins the parts of a row: weights 2^(lse_i - max), then their mean.  One warp
+// a row, four channels a lane.
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int rows_per_tile) {
+  const int rows = p.G * p.Lq;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= (long long)p.B * p.Hkv * rows) return;
+  const int bh = (int)(row / rows), r = (int)(row - (long long)bh * rows);
+  const int b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  int len = p.max_len;
+  if (p.lengths != nullptr) len = min(max(p.lengths[b], 0), p.max_len);
+  // the parts that this row's tile wrote (part 0 always is)
+  const int last_row = min(r / rows_per_tile * rows_per_tile + rows_per_tile, rows) - 1;
+  const int end = row_limit(p, last_row, len);
+  const int per = tiles_per_split(end, p.n_split);
+  const int n = per == 0 ? 1 : ((end + kTok - 1) / kTok + per - 1) / per;
+  const float* lse = p.part_lse + row * p.n_split;
+  const float4* po = reinterpret_cast<const float4*>(p.part_o + row * p.n_split * kD) + lane;
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, lse[i]);
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+  const float mb = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float w = ex2_approx(lse[i] - mb);
+    const float4 x = po[(long long)i * 32];
+    l += w;
+    acc.x += w * x.x;
+    acc.y += w * x.y;
+    acc.z += w * x.z;
+    acc.w += w * x.w;
+  }
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+  const int i = r / p.G, hq = kvh * p.G + r - i * p.G, Hq = p.Hkv * p.G;
+  const long long at = (((long long)b * p.Lq + i) * Hq + hq) * kD + 4 * lane;
+  acc.x = l == 0.f ? 0.f : acc.x * f;
+  acc.y = l == 0.f ? 0.f : acc.y * f;
+  acc.z = l == 0.f ? 0.f : acc.z * f;
+  acc.w = l == 0.f ? 0.f : acc.w * f;
+  uint2 v;
+  if (p.f16) {
+    v.x = as_u32(__floats2half2_rn(acc.x, acc.y));
+    v.y = as_u32(__floats2half2_rn(acc.z, acc.w));
+  } else {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x, acc.y), y = __floats2bfloat162_rn(acc.z, acc.w);
+    v.x = *reinterpret_cast<const uint32_t*>(&x);
+    v.y = *reinterpret_cast<const uint32_t*>(&y);
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = v;
+  if (lane == 0) p.lse[((long long)b * Hq + hq) * p.Lq + i] = lse2 * 0.69314718055994531f;
+}
+
+// Resident CTAs an SM that the split is planned for.
+constexpr int kResident = 2;
+
+struct Plan {
+  int nt, n_rt, n_split;
+};
+
+// Parts of a sequence: the count that ends first when `units` x parts CTAs run
+// in waves, a part costing its tokens plus a fixed start and end.
+Plan plan(int B, int Hkv, long long rows, int max_len) {
+  Plan r;
+  r.nt = rows <= 8 ? 1 : 2;
+  r.n_rt = (int)((rows + 8 * r.nt - 1) / (8 * r.nt));
+  const long long units = (long long)B * Hkv * r.n_rt, slots = (long long)sm_count() * kResident;
+  const int tiles = (max_len + kTok - 1) / kTok;
+  double best = 0;
+  r.n_split = 1;
+  for (int n = 1; n <= 256 && n * kWarps <= (tiles > kWarps ? tiles : kWarps); ++n) {
+    const long long waves = (units * n + slots - 1) / slots;
+    const double cost = (double)waves * ((tiles + n - 1) / n + 12) + (n > 1 ? 16 : 0);
+    if (n == 1 || cost < best) {
+      best = cost;
+      r.n_split = n;
+    }
+  }
+  return r;
+}
+
+template <int kBits, int kG, int kNT>
+cudaError_t launch_few(const AttnParams& p, long long blocks, cudaStream_t s) {
+  using St = Stage<kBits, kG>;
+  constexpr uint32_t ring = kWarps * St::kCount * St::kBytes, join = kWarps * 8 * kNT * kD * 4;
+  constexpr uint32_t smem = ring > join ? ring : join;
+  auto kern = attn_few_kernel<kBits, kG, kNT>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  kern<<<(unsigned)blocks, kAttnThreads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+template <int kBits, int kG>
+cudaError_t launch_nt(int nt, const AttnParams& p, long long blocks, cudaStream_t s) {
+  return nt == 1 ? launch_few<kBits, kG, 1>(p, blocks, s) : launch_few<kBits, kG, 2>(p, blocks, s);
+}
+
+}  // namespace kvq
+}  // namespace core
+
+using namespace core;
+
+namespace {
+template <class C>
+void carve_parts(C& c, int n_split, long long rows, float** o, float** lse) {
+  if (n_split <= 1) return;
+  *o = c.template take<float>((size_t)rows * n_split * kvq::kD);
+  *lse = c.template take<float>((size_t)rows * n_split);
+}
+struct SizerOut : Sizer {
+  template <class T>
+  T* take(size_t n) {
+    Sizer::take<T>(n);
+    return nullptr;
+  }
+};
+}  // namespace
+
+extern "C" size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries,
+                                                     int32_t max_length) {
+  if (cache == nullptr || cache->n_kv_heads <= 0 || n_q_heads < cache->n_kv_heads || n_queries <= 0 ||
+      cache->batch <= 0 || max_length < 0)
+    return 0;
+  const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
+  const kvq::Plan pl = kvq::plan(cache->batch, cache->n_kv_heads, rows, max_length);
+  SizerOut z;
+  float *a, *b;
+  carve_parts(z, pl.n_split, rows * cache->batch * cache->n_kv_heads, &a, &b);
+  return z.used;
+}
+
+extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_t n_q_heads, int32_t n_queries,
+                                  const void* q, const int64_t* q_strides, const int32_t* lengths,
+                                  int32_t max_length, const uint8_t* key_mask, int64_t mask_stride, int32_t causal,
+                                  float softmax_scale, void* out, float* lse, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const char* fn = "core_kvq_attention";
+  int rc = check_kvq(cache, fn);
+  if (rc != CORE_OK) return rc;
+  const std::string f(fn);
+  if (q == nullptr || q_strides == nullptr || out == nullptr || lse == nullptr)
+    return set_error(CORE_ERR_INVALID_ARG, f + ": NULL argument");
+  if (n_q_heads <= 0 || n_queries <= 0) return set_error(CORE_ERR_INVALID_ARG, f + ": non-positive dimension");
+  if (n_q_heads % cache->n_kv_heads != 0)
+    return set_error(CORE_ERR_INVALID_ARG, f + ": n_q_heads must be a multiple of n_kv_heads");
+  if (dtype != CORE_DTYPE_BF16 && dtype != CORE_DTYPE_F16)
+    return set_error(CORE_ERR_UNSUPPORTED, f + ": dtype must be bf16 or f16");
+  if (max_length < 0 || max_length > cache->capacity)
+    return set_error(CORE_ERR_INVALID_ARG, f + ": max_length outside the cache's capacity");
+  if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale))
+    return set_error(CORE_ERR_INVALID_ARG, f + ": softmax_scale must be positive");
+  if (!aligned16(q) || !aligned16(out)) return set_error(CORE_ERR_INVALID_ARG, f + ": q and out must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] % 8 != 0) return set_error(CORE_ERR_INVALID_ARG, f + ": q strides must be multiples of 8 elements");
+  if (key_mask != nullptr && mask_stride < max_length)
+    return set_error(CORE_ERR_INVALID_ARG, f + ": key_mask rows shorter than max_length");
+  const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
+  if (rows > INT_MAX / 2) return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
+
+  kvq::AttnParams p{};
+  p.kc = static_cast<const uint8_t*>(cache->k_codes);
+  p.km = static_cast<const uint32_t*>(cache->k_meta);
+  p.vc = static_cast<const uint8_t*>(cache->v_codes);
+  p.vm = static_cast<const uint32_t*>(cache->v_meta);
+  p.q = q;
+  p.qb = q_strides[0];
+  p.qh = q_strides[1];
+  p.ql = q_strides[2];
+  p.lengths = lengths;
+  p.mask = key_mask;
+  p.mask_stride = mask_stride;
+  p.B = cache->batch;
+  p.Hkv = cache->n_kv_heads;
+  p.G = n_q_heads / cache->n_kv_heads;
+  p.Lq = n_queries;
+  p.cap = cache->capacity;
+  p.max_len = max_length;
+  p.causal = causal != 0;
+  p.f16 = dtype == CORE_DTYPE_F16;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.out = out;
+  p.lse = lse;
+  p.status = device_status();
+  const kvq::Plan pl = kvq::plan(p.B, p.Hkv, rows, max_length);
+  p.n_rt = pl.n_rt;
+  p.n_split = pl.n_split;
+  Carver c(workspace, workspace_bytes);
+  carve_parts(c, pl.n_split, rows * p.B * p.Hkv, &p.part_o, &p.part_lse);
+  if (c.overflow) return set_error(CORE_ERR_WORKSPACE, f + ": workspace too small");
+  const long long blocks = (long long)p.B * p.Hkv * pl.n_rt * pl.n_split;
+  const long long join_blocks = (rows * p.B * p.Hkv + 3) / 4;
+  if (blocks > INT_MAX || join_blocks > INT_MAX)
+    return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (cache->bits == 4)
+    e = cache->group == 32   ? kvq::launch_nt<4, 4>(pl.nt, p, blocks, s)
+        : cache->group == 64 ? kvq::launch_nt<4, 2>(pl.nt, p, blocks, s)
+                             : kvq::launch_nt<4, 1>(pl.nt, p, blocks, s);
+  else
+    e = cache->group == 32   ? kvq::launch_nt<8, 4>(pl.nt, p, blocks, s)
+        : cache->group == 64 ? kvq::launch_nt<8, 2>(pl.nt, p, blocks, s)
+                             : kvq::launch_nt<8, 1>(pl.nt, p, blocks, s);
+  if (e != cudaSuccess) return cuda_error(e, "attn_few_kernel launch");
+  if (pl.n_split > 1) {
+    kvq::attn_join_kernel<<<(unsigned)join_blocks, 128, 0, s>>>(p, 8 * pl.nt);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_error(e, "attn_join_kernel launch");
+  }
+  return CORE_OK;
+}

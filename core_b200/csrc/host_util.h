@@ -68,5 +68,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 // Validates the shared dimensions; f32 caches pass only where allow_f32.
 int check_dims(const core_dims_t* d, const char* fn, bool allow_f32 = false);
+// Validates a quantised cache's buffers and dimensions.
+int check_kvq(const core_kvq_t* c, const char* fn);
 
 }  // namespace core

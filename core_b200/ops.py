@@ -160,6 +160,162 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     return out, lse
 
 
+# ---------------------------------------------------------------------------
+# Quantised KV cache (core_b200.kvcache.QuantizedKV)
+# ---------------------------------------------------------------------------
+
+_KVQ_DTYPES = _READOUT_DTYPES
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """t itself where its last dim is contiguous and its base and other strides
+    are 16-byte aligned, else a contiguous copy."""
+    size = t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _per_sequence(value, cache, name: str):
+    """(pointer to (B,) int32 on the device, scalar) of an int or a tensor."""
+    if not isinstance(value, torch.Tensor):
+        return None, int(value)
+    if value.shape != (cache.batch,) or value.dtype != torch.int32 or not value.is_contiguous():
+        raise ValueError(f"{name} must be an int or a contiguous (B,) int32 tensor")
+    if value.device != cache.device:
+        raise ValueError(f"{name} must be on the cache's device")
+    return value.data_ptr(), 0
+
+
+def _row_index(index, cache, name: str):
+    if index.dim() != 2 or index.shape[0] != cache.batch:
+        raise ValueError(f"{name} must be (B, n)")
+    if index.device != cache.device:
+        raise ValueError(f"{name} must be on the cache's device")
+    return index.to(torch.int32).contiguous()
+
+
+def kv_quantize(keys: torch.Tensor, values: torch.Tensor, cache, start, *,
+                index: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
+    """Quantise rows of K and V into ``cache`` (a ``kvcache.QuantizedKV``).
+
+    keys, values: (B, Hkv, L, 128), bf16, f16 or f32, any strides.  Row t of
+    sequence b goes to slot ``start`` + t; ``start`` is an int or a (B,) int32
+    device tensor.  ``index`` (B, n) picks the source rows (a selection's kept
+    rows are compacted and quantised in one pass); ``counts`` (B,) int32 writes
+    only the first counts[b] rows.  Slots or source rows out of range are
+    skipped and reported by :func:`status`.
+    """
+    _require_cuda(keys, values, index, counts)
+    code = _KVQ_DTYPES.get(keys.dtype)
+    if code is None or values.dtype != keys.dtype:
+        raise TypeError("kv_quantize takes keys and values of one dtype, bf16, f16 or f32")
+    if (keys.dim() != 4 or keys.shape != values.shape or keys.shape[0] != cache.batch
+            or keys.shape[1] != cache.n_kv_heads or keys.shape[3] != HEAD_DIM):
+        raise ValueError(f"keys and values must be ({cache.batch}, {cache.n_kv_heads}, L, {HEAD_DIM})")
+    if keys.device != cache.device or values.device != cache.device:
+        raise ValueError("keys and values must be on the cache's device")
+    keys, values = _aligned_rows(keys), _aligned_rows(values)
+    n = L = keys.shape[2]
+    if index is not None:
+        index = _row_index(index, cache, "index")
+        n = index.shape[1]
+    if n == 0:
+        return
+    at, at0 = _per_sequence(start, cache, "start")
+    cnt = None if counts is None else _per_sequence(counts, cache, "counts")[0]
+    ks, vs = keys.stride(), values.stride()
+    check(_lib.load().core_kvq_quantize(
+        cache.handle, code, keys.data_ptr(), (ctypes.c_int64 * 3)(*ks[:3]), values.data_ptr(),
+        (ctypes.c_int64 * 3)(*vs[:3]), L, n, None if index is None else index.data_ptr(), at, at0,
+        cnt, _stream(cache.device)))
+
+
+def kv_dequantize(cache, *, start=0, count: int | None = None, index: torch.Tensor | None = None,
+                  dtype: torch.dtype = torch.bfloat16):
+    """(keys, values) (B, Hkv, n, 128) read back from ``cache``: ``count`` slots
+    from ``start`` (an int or a (B,) int32 device tensor), or the slots ``index``
+    (B, n).  Each value is n s + z rounded once to ``dtype`` (bf16, f16, f32)."""
+    code = _KVQ_DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"kv_dequantize gives bf16, f16 or f32; got {dtype}")
+    _require_cuda(index)
+    at, at0 = None, 0
+    if index is not None:
+        index = _row_index(index, cache, "index")
+        n = index.shape[1]
+    else:
+        if count is None or count < 0:
+            raise ValueError("kv_dequantize needs index, or a count of slots")
+        n = int(count)
+        at, at0 = _per_sequence(start, cache, "start")
+    shape = (cache.batch, cache.n_kv_heads, n, HEAD_DIM)
+    k = torch.empty(shape, dtype=dtype, device=cache.device)
+    v = torch.empty(shape, dtype=dtype, device=cache.device)
+    if n:
+        check(_lib.load().core_kvq_dequantize(
+            cache.handle, code, n, None if index is None else index.data_ptr(), at, at0,
+            k.data_ptr(), v.data_ptr(), _stream(cache.device)))
+    return k, v
+
+
+def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | None = None,
+                        key_mask: torch.Tensor | None = None, softmax_scale: float | None = None,
+                        causal: bool = True, out: torch.Tensor | None = None):
+    """Attention of q over a quantised cache, read as codes.
+
+    q: (B, Hq, Lq, 128), bf16 or f16, any strides; Hq a multiple of the cache's
+    KV heads.  ``lengths``: tokens of each sequence, an int or a (B,) int32 device
+    tensor; ``max_length``: a host-side bound of them (default: the capacity).
+    The queries are the sequence's last ones (``causal``; query i sees the tokens
+    before lengths - Lq + i + 1) or see every token (``causal=False``).
+    ``key_mask`` (B, n >= max_length) bool or uint8: False hides a token.
+    Returns (out (B, Lq, Hq, 128) in q's dtype, lse (B, Hq, Lq) f32); a row that
+    sees no token gives 0 and -inf.
+    """
+    _require_cuda(q, key_mask)
+    code = _ATTN_DTYPES.get(q.dtype)
+    if code is None:
+        raise TypeError(f"attention_quantized takes bf16 or f16 queries; got {q.dtype}")
+    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != HEAD_DIM or q.shape[1] % cache.n_kv_heads:
+        raise ValueError(f"q must be ({cache.batch}, Hq, Lq, {HEAD_DIM}) with Hq a multiple of "
+                         f"{cache.n_kv_heads}")
+    if q.device != cache.device:
+        raise ValueError("q must be on the cache's device")
+    q = _aligned_rows(q)
+    B, Hq, Lq, _ = q.shape
+    at, n = _per_sequence(lengths, cache, "lengths")
+    if at is not None:
+        n = cache.capacity if max_length is None else int(max_length)
+    mask, mask_stride = None, 0
+    if key_mask is not None:
+        if (key_mask.dim() != 2 or key_mask.shape[0] != B or key_mask.shape[1] < n
+                or key_mask.dtype not in (torch.bool, torch.uint8)):
+            raise ValueError("key_mask must be a (B, >= max_length) bool or uint8 tensor")
+        if key_mask.device != cache.device:
+            raise ValueError("key_mask must be on the cache's device")
+        if key_mask.stride(1) != 1 or (B > 1 and key_mask.stride(0) < key_mask.shape[1]):
+            key_mask = key_mask.contiguous()
+        mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if B > 1 else key_mask.shape[1]
+    if out is None:
+        out = torch.empty((B, Lq, Hq, HEAD_DIM), dtype=q.dtype, device=q.device)
+    elif out.shape != (B, Lq, Hq, HEAD_DIM) or not out.is_contiguous() or out.dtype != q.dtype:
+        raise ValueError("out must be a contiguous (B, Lq, Hq, 128) tensor of q's dtype")
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
+    if Lq == 0:
+        return out, lse
+    lib = _lib.load()
+    need = lib.core_kvq_attention_workspace_bytes(cache.handle, Hq, Lq, n)
+    ws = _workspace(need, q.device) if need else None
+    scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
+    st = q.stride()
+    check(lib.core_kvq_attention(
+        cache.handle, code, Hq, Lq, q.data_ptr(), (ctypes.c_int64 * 3)(*st[:3]), at, n, mask,
+        mask_stride, 1 if causal else 0, scale, out.data_ptr(), lse.data_ptr(),
+        None if ws is None else ws.data_ptr(), need, _stream(q.device)))
+    return out, lse
+
+
 def split_bf16(w: torch.Tensor, terms: int) -> torch.Tensor:
     """f32 -> (terms, *w.shape) bf16 whose sum reproduces w (hi, mid, lo)."""
     _require_cuda(w)

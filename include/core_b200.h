@@ -47,7 +47,7 @@ extern "C" {
 /* ---- dtypes ---- */
 #define CORE_DTYPE_BF16 1
 #define CORE_DTYPE_F32 2
-#define CORE_DTYPE_F16 3 /* core_rope_queries and core_compact_kv only */
+#define CORE_DTYPE_F16 3 /* where an entry point says so */
 
 typedef struct core_dims {
   int32_t batch;      /* B   */
@@ -441,6 +441,80 @@ int core_attention_prefill(const core_dims_t* dims, const void* q, const int64_t
                            const void* k, const int64_t* k_strides, const void* v,
                            const int64_t* v_strides, void* out, float* lse, float softmax_scale,
                            void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Quantised KV cache: K and V rows held in 4 or 8 bits.  No reference
+ * counterpart (the reference stores its kept rows in the model's dtype).
+ *
+ * A row is one token of one KV head, 128 channels.  Each group of `group`
+ * neighbouring channels has an f16 scale s and zero z; a code n stands for
+ * n s + z:  lo, hi = least and greatest value of the group within +-61440,
+ * z = f16(lo), s = f16((hi - lo) / N), n = rint((x - z) / s) kept in 0..N,
+ * N = 15 or 255 (each step rounded once in f32).  Values beyond +-61440
+ * saturate; a group that holds a NaN reads back as NaN.
+ *   codes : (B, Hkv, capacity, 16 * bits) bytes
+ *   meta  : (B, Hkv, capacity, 128 / group, 2) f16, (s, z)
+ * capacity is a multiple of 128; all four buffers are 16-byte aligned and may
+ * start uninitialised (nothing beyond a sequence's length is interpreted).
+ * Order inside a row: a 32-bit word holds neighbouring channels, even ones in
+ * its low half (4 bits, nibbles from the lowest: e0 e2 e4 e6 e1 e3 e5 e7;
+ * 8 bits, bytes: e0 e2 e1 e3).  K, 4 bits: channels 32 b + 8 t .. + 7 are word
+ * 4 t + b.  K, 8 bits: channels 32 b + 8 t + 4 h .. + 3 are word
+ * 16 (b / 2) + 4 t + 2 (b % 2) + h, its index xor 16 for odd tokens.  V: words
+ * in channel order, the index xor 8 for tokens with bit 1 set (4 bits), xor
+ * 8 (token % 4) (8 bits).
+ * ------------------------------------------------------------------------- */
+typedef struct core_kvq {
+  void* k_codes;
+  void* k_meta;
+  void* v_codes;
+  void* v_meta;
+  int32_t batch;      /* B */
+  int32_t n_kv_heads; /* Hkv */
+  int32_t capacity;   /* tokens a sequence has room for */
+  int32_t bits;       /* 4 or 8 */
+  int32_t group;      /* 32, 64 or 128 */
+} core_kvq_t;
+
+/* Writes n_rows rows of K and V per sequence into slots start[b] + t (start
+ * NULL: start_all + t), t = 0 .. min(counts[b], n_rows) - 1 (counts NULL: all).
+ *   k, v    : rows (b, h, l) at the given element strides, 128 contiguous
+ *             channels each, 16-byte aligned; dtype CORE_DTYPE_BF16, F16 or F32
+ *   index   : optional (B, n_rows) source rows l (a selection's kept rows);
+ *             NULL: row t
+ * A slot or source row out of range is skipped and recorded as
+ * CORE_ERR_INVALID_ARG (device status sites 1401, 1402). */
+int core_kvq_quantize(const core_kvq_t* cache, int32_t dtype, const void* k, const int64_t* k_strides,
+                      const void* v, const int64_t* v_strides, int32_t src_len, int32_t n_rows,
+                      const int32_t* index, const int32_t* start, int32_t start_all,
+                      const int32_t* counts, void* stream);
+
+/* Reads rows back as n s + z, rounded once: slots index[b, t], or start[b] + t
+ * (start NULL: start_all + t), into out_k, out_v (B, Hkv, n_rows, 128) of
+ * dtype CORE_DTYPE_BF16, F16 or F32.  A slot out of range gives zeros and
+ * records CORE_ERR_INVALID_ARG (site 1411). */
+int core_kvq_dequantize(const core_kvq_t* cache, int32_t dtype, int32_t n_rows, const int32_t* index,
+                        const int32_t* start, int32_t start_all, void* out_k, void* out_v, void* stream);
+
+/* Attention over the cache.
+ *   q        : (B, n_q_heads, n_queries, 128) at the given element strides
+ *              (multiples of 8), bf16 or f16; n_q_heads a multiple of n_kv_heads
+ *   lengths  : (B) tokens of each sequence, 0 .. max_length (NULL: max_length
+ *              for all); one outside is clamped and recorded (site 1421)
+ *   key_mask : optional (B, mask_stride) bytes, 0 hides a token
+ *   causal   : query i sees the tokens before lengths[b] - n_queries + i + 1;
+ *              0: all of them
+ *   out      : (B, n_queries, n_q_heads, 128) in q's dtype
+ *   lse      : (B, n_q_heads, n_queries) f32, natural log
+ * A row that sees no token gives 0 and -inf.  Hidden tokens count for nothing
+ * whatever their bytes hold. */
+size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries,
+                                          int32_t max_length);
+int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_t n_q_heads, int32_t n_queries,
+                       const void* q, const int64_t* q_strides, const int32_t* lengths,
+                       int32_t max_length, const uint8_t* key_mask, int64_t mask_stride, int32_t causal,
+                       float softmax_scale, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,34 @@
+"""Host-side checks of the quantised KV cache: what its entry points refuse
+without touching a GPU."""
+
+import ctypes
+
+from core_b200 import _lib
+
+def test_quantised_cache_arguments_rejected_on_host():
+    """The quantised-cache entry points refuse bad shapes before any CUDA call."""
+    lib = _lib.load()
+    s = ctypes.cast((ctypes.c_int64 * 3)(1 << 20, 1 << 14, 128), ctypes.c_void_p)
+    p, bad = ctypes.c_void_p(256), ctypes.c_void_p(264)
+
+    def cache(k=256, bits=4, group=64, cap=128, heads=2):
+        return ctypes.byref(_lib.CoreKvq(k, 256, 256, 256, 1, heads, cap, bits, group))
+
+    def write(c, k=p, n=4, start=0, dtype=_lib.CORE_DTYPE_BF16):
+        return lib.core_kvq_quantize(c, dtype, k, s, p, s, 4, n, None, None, start, None, None)
+
+    assert write(cache(k=None)) == -1 and write(cache(bits=3)) == -2 and write(cache(group=16)) == -2
+    assert write(cache(cap=100)) == -1 and write(cache(k=264)) == -1 and write(cache(), k=bad) == -1
+    assert write(cache(), n=5) == -1 and write(cache(), n=0) == -1 and write(cache(), start=125) == -1
+    assert lib.core_kvq_dequantize(cache(), 1, 4, None, None, 126, p, p, None) == -1
+    assert lib.core_kvq_dequantize(cache(), 1, 4, None, None, 0, p, bad, None) == -1
+
+    def attend(c, hq=4, lq=1, n=64, dtype=_lib.CORE_DTYPE_BF16, q=p, scale=0.1, mask=None, ms=0):
+        return lib.core_kvq_attention(c, dtype, hq, lq, q, s, None, n, mask, ms, 1, scale, p, p, None, 0, None)
+
+    assert attend(cache(), hq=3) == -1 and attend(cache(), lq=0) == -1 and attend(cache(), n=129) == -1
+    assert attend(cache(), dtype=_lib.CORE_DTYPE_F32) == -2 and attend(cache(), q=bad) == -1
+    assert attend(cache(), scale=-1.0) == -1 and attend(cache(), mask=p, ms=63) == -1
+    assert "key_mask" in _lib.last_error()
+    # one KV head's long sequence is cut into parts: the workspace is missing
+    assert attend(cache(cap=4096, heads=1), hq=1, n=4096) == -6
