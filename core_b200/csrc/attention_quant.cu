@@ -30,9 +30,8 @@
 #include <climits>
 #include <cmath>
 
-#include "common.cuh"
+#include "attention_quant.cuh"
 #include "host_util.h"
-#include "kvq_common.cuh"
 
 namespace core {
 namespace kvq {
@@ -40,28 +39,7 @@ namespace kvq {
 constexpr int kWarps = 4;
 constexpr int kAttnThreads = kWarps * 32;
 constexpr int kTok = 32;  // tokens of a warp's tile
-constexpr float kRaise = 8.0f;  // P <= 2^8 before the maximum is raised
 
-struct AttnParams {
-  const uint8_t* kc;
-  const uint32_t* km;
-  const uint8_t* vc;
-  const uint32_t* vm;
-  const void* q;
-  long long qb, qh, ql;  // element strides of (B, Hq, Lq)
-  const int* lengths;    // (B), or null: max_len for all
-  const uint8_t* mask;   // (B, mask_stride), 0: hidden; or null
-  long long mask_stride;
-  int B, Hkv, G, Lq, cap, max_len;
-  int n_rt, n_split;  // row tiles a KV head, parts of a sequence
-  int causal, f16;
-  float scale_log2;
-  void* out;    // (B, Lq, Hq, d)
-  float* lse;   // (B, Hq, Lq), natural log
-  float* part_o;    // (B Hkv, row, split, d) f32 where n_split > 1
-  float* part_lse;  // (B Hkv, row, split), base 2
-  DeviceStatus* status;
-};
 
 template <int kBits, int kG>
 struct Stage {
@@ -69,34 +47,6 @@ struct Stage {
   static constexpr uint32_t kKc = 0, kVc = kCodes, kKm = 2 * kCodes, kVm = kKm + kMeta, kBytes = kVm + kMeta;
   static constexpr int kCount = kBits == 4 ? 4 : 3;
 };
-
-// Tokens of one sequence that the kernel sees.
-__device__ __forceinline__ int sequence_length(const AttnParams& p, int b) {
-  int n = p.max_len;
-  if (p.lengths != nullptr) {
-    const int given = p.lengths[b];
-    if (given < 0 || given > p.max_len) {
-      if (threadIdx.x == 0) record_error(p.status, CORE_ERR_INVALID_ARG, 1421, b);
-      n = given < 0 ? 0 : p.max_len;
-    } else {
-      n = given;
-    }
-  }
-  return n;
-}
-
-// Last token (exclusive) that query row r of a KV head sees; rows past the end see none.
-__device__ __forceinline__ int row_limit(const AttnParams& p, int r, int len) {
-  const int i = r / p.G;
-  if (i >= p.Lq) return 0;
-  return p.causal ? max(len - p.Lq + i + 1, 0) : len;
-}
-
-// Warp tiles of a sequence and the ones of a part.
-__device__ __forceinline__ int tiles_per_split(int end, int n_split) {
-  const int tiles = (end + kTok - 1) / kTok;
-  return (tiles + n_split - 1) / n_split;
-}
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -157,11 +107,7 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, int b, int kvh
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float2 f;
-      if (p.f16)
-        f = __half22float2(as_half2(w[j]));
-      else
-        f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+      const float2 f = query_pair(w[j], p.f16 != 0);
       x[8 * c + 2 * j] = f.x;
       x[8 * c + 2 * j + 1] = f.y;
       mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
@@ -169,19 +115,14 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, int b, int kvh
   }
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  // power of two that brings the row's largest element into [2^7, 2^8); the two
-  // factors keep it within f32 for any exponent
-  const int e = (int)((__float_as_uint(mx) >> 23) & 255u) - 127;
-  const int sh = mx > 0.f && e < 128 ? 7 - e : 0;
-  const int sh1 = sh / 2, sh2 = sh - sh1;
-  const float f1 = __uint_as_float((uint32_t)(127 + sh1) << 23), f2 = __uint_as_float((uint32_t)(127 + sh2) << 23);
+  const RowShift sh = row_shift(mx);
   float part[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     part[c] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const __half2 h = __floats2half2_rn(x[8 * c + 2 * j] * f1 * f2, x[8 * c + 2 * j + 1] * f1 * f2);
+      const __half2 h = __floats2half2_rn(x[8 * c + 2 * j] * sh.f1 * sh.f2, x[8 * c + 2 * j + 1] * sh.f1 * sh.f2);
       const float2 r = __half22float2(h);
       part[c] += r.x + r.y;
       // 4 bits: odd pairs meet 16 n
@@ -200,9 +141,8 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, int b, int kvh
     s = t == 0 ? (part[0] + part[1]) + (part[2] + part[3]) : 0.f;
   const __half hi = __float2half_rn(s);
   qsum = as_u32(__halves2half2(hi, __float2half_rn(s - __half2float(hi))));
-  // S = raw * row_scale with raw in units of 2^-24 2^sh
-  row_scale = p.scale_log2 * 16777216.f;
-  row_scale = row_scale * __uint_as_float((uint32_t)(127 - sh1) << 23) * __uint_as_float((uint32_t)(127 - sh2) << 23);
+  // the sums of products come in units of 2^-24 (the codes') and of the shift
+  row_scale = p.scale_log2 * 16777216.f * sh.inv1 * sh.inv2;
 }
 
 template <int kBits, int kG, int kNT>
@@ -235,7 +175,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_few_kernel(const AttnParams
   const int last_row = min(row0 + 8 * kNT, rows) - 1;
   const int end = row_limit(p, last_row, len);  // no row of the tile sees a token from here on
   const int first_end = row_limit(p, row0, len);  // every row sees the tokens before this
-  const int per = tiles_per_split(end, p.n_split);
+  const int per = tiles_per_split(end, kTok, p.n_split);
   const int tile0 = split * per, tile1 = min(tile0 + per, (end + kTok - 1) / kTok);
   if (p.n_split > 1 && tile0 >= tile1 && split > 0) return;  // the join does not read this part
 
@@ -582,7 +522,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_few_kernel(const AttnParams
 
 // Joins the parts of a row: weights 2^(lse_i - max), then their mean.  One warp
 // a row, four channels a lane.
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int rows_per_tile) {
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int rows_per_tile, int tok) {
   const int rows = p.G * p.Lq;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -594,8 +534,8 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int 
   // the parts that this row's tile wrote (part 0 always is)
   const int last_row = min(r / rows_per_tile * rows_per_tile + rows_per_tile, rows) - 1;
   const int end = row_limit(p, last_row, len);
-  const int per = tiles_per_split(end, p.n_split);
-  const int n = per == 0 ? 1 : ((end + kTok - 1) / kTok + per - 1) / per;
+  const int per = tiles_per_split(end, tok, p.n_split);
+  const int n = per == 0 ? 1 : ((end + tok - 1) / tok + per - 1) / per;
   const float* lse = p.part_lse + row * p.n_split;
   const float4* po = reinterpret_cast<const float4*>(p.part_o + row * p.n_split * kD) + lane;
   float m = -INFINITY;
@@ -640,22 +580,29 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int 
 constexpr int kResident = 2;
 
 struct Plan {
+  bool many;
   int nt, n_rt, n_split;
 };
+
+// Query rows a KV head from which the tcgen05 kernel (256-row tiles) takes over.
+constexpr int kManyFrom = 33;
 
 // Parts of a sequence: the count that ends first when `units` x parts CTAs run
 // in waves, a part costing its tokens plus a fixed start and end.
 Plan plan(int B, int Hkv, long long rows, int max_len) {
   Plan r;
+  r.many = rows >= kManyFrom;
   r.nt = rows <= 8 ? 1 : 2;
-  r.n_rt = (int)((rows + 8 * r.nt - 1) / (8 * r.nt));
-  const long long units = (long long)B * Hkv * r.n_rt, slots = (long long)sm_count() * kResident;
-  const int tiles = (max_len + kTok - 1) / kTok;
+  const int per_tile = r.many ? kManyRows : 8 * r.nt, tok = r.many ? kManyTok : kTok, least = r.many ? 1 : kWarps;
+  r.n_rt = (int)((rows + per_tile - 1) / per_tile);
+  const long long units = (long long)B * Hkv * r.n_rt, slots = (long long)sm_count() * (r.many ? 1 : kResident);
+  const int tiles = (max_len + tok - 1) / tok;
+  const double fixed = r.many ? 4 : 12, join = r.many ? 4 : 16;
   double best = 0;
   r.n_split = 1;
-  for (int n = 1; n <= 256 && n * kWarps <= (tiles > kWarps ? tiles : kWarps); ++n) {
+  for (int n = 1; n <= 256 && n * least <= (tiles > least ? tiles : least); ++n) {
     const long long waves = (units * n + slots - 1) / slots;
-    const double cost = (double)waves * ((tiles + n - 1) / n + 12) + (n > 1 ? 16 : 0);
+    const double cost = (double)waves * ((tiles + n - 1) / n + fixed) + (n > 1 ? join : 0);
     if (n == 1 || cost < best) {
       best = cost;
       r.n_split = n;
@@ -779,7 +726,9 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
     return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (cache->bits == 4)
+  if (pl.many)
+    e = kvq::launch_many(cache->bits, cache->group, p, blocks, s);
+  else if (cache->bits == 4)
     e = cache->group == 32   ? kvq::launch_nt<4, 4>(pl.nt, p, blocks, s)
         : cache->group == 64 ? kvq::launch_nt<4, 2>(pl.nt, p, blocks, s)
                              : kvq::launch_nt<4, 1>(pl.nt, p, blocks, s);
@@ -787,9 +736,10 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
     e = cache->group == 32   ? kvq::launch_nt<8, 4>(pl.nt, p, blocks, s)
         : cache->group == 64 ? kvq::launch_nt<8, 2>(pl.nt, p, blocks, s)
                              : kvq::launch_nt<8, 1>(pl.nt, p, blocks, s);
-  if (e != cudaSuccess) return cuda_error(e, "attn_few_kernel launch");
+  if (e != cudaSuccess) return cuda_error(e, pl.many ? "attn_many_kernel launch" : "attn_few_kernel launch");
   if (pl.n_split > 1) {
-    kvq::attn_join_kernel<<<(unsigned)join_blocks, 128, 0, s>>>(p, 8 * pl.nt);
+    kvq::attn_join_kernel<<<(unsigned)join_blocks, 128, 0, s>>>(p, pl.many ? kvq::kManyRows : 8 * pl.nt,
+                                                                         pl.many ? kvq::kManyTok : kvq::kTok);
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_error(e, "attn_join_kernel launch");
   }
   return CORE_OK;
