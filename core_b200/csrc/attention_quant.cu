@@ -45,7 +45,7 @@ template <int kBits, int kG>
 struct Stage {
   static constexpr uint32_t kCodes = kTok * 16 * kBits, kMeta = kTok * 4 * kG;
   static constexpr uint32_t kKc = 0, kVc = kCodes, kKm = 2 * kCodes, kVm = kKm + kMeta, kBytes = kVm + kMeta;
-  static constexpr int kCount = kBits == 4 ? 4 : 3;
+  static constexpr int kCount = kBits == 4 ? (kG == 4 ? 2 : 3) : 2;
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -146,7 +146,7 @@ __device__ __forceinline__ void load_queries(const AttnParams& p, int b, int kvh
 }
 
 template <int kBits, int kG, int kNT>
-__global__ void __launch_bounds__(kAttnThreads) attn_few_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kernel(const AttnParams p) {
   using St = Stage<kBits, kG>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps * St::kCount];
@@ -520,13 +520,17 @@ __global__ void __launch_bounds__(kAttnThreads) attn_few_kernel(const AttnParams
   }
 }
 
-// Joins the parts of a row: weights 2^(lse_i - max), then their mean.  One warp
-// a row, four channels a lane.
+// Joins the parts of a row: weights 2^(lse_i - max), then their mean.  A CTA of
+// four warps takes a row: every warp works out the weights, takes every fourth
+// part, four channels a lane, and the four sums meet in shared memory.
+constexpr int kMaxSplit = 128;
+
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int rows_per_tile, int tok) {
+  __shared__ float weight[kMaxSplit];
+  __shared__ float4 sums[4][32];
   const int rows = p.G * p.Lq;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= (long long)p.B * p.Hkv * rows) return;
+  const long long row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bh = (int)(row / rows), r = (int)(row - (long long)bh * rows);
   const int b = bh / p.Hkv, kvh = bh - b * p.Hkv;
   int len = p.max_len;
@@ -537,47 +541,66 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int 
   const int per = tiles_per_split(end, tok, p.n_split);
   const int n = per == 0 ? 1 : ((end + tok - 1) / tok + per - 1) / per;
   const float* lse = p.part_lse + row * p.n_split;
-  const float4* po = reinterpret_cast<const float4*>(p.part_o + row * p.n_split * kD) + lane;
+  float v[kMaxSplit / 32];
   float m = -INFINITY;
-  for (int i = lane; i < n; i += 32) m = fmaxf(m, lse[i]);
+#pragma unroll
+  for (int k = 0; k < kMaxSplit / 32; ++k) {
+    v[k] = 32 * k + lane < n ? lse[32 * k + lane] : -INFINITY;
+    m = fmaxf(m, v[k]);
+  }
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
   const float mb = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float w = ex2_approx(lse[i] - mb);
-    const float4 x = po[(long long)i * 32];
+#pragma unroll
+  for (int k = 0; k < kMaxSplit / 32; ++k) {
+    const float w = ex2_approx(v[k] - mb);
     l += w;
+    if (warp == 0) weight[32 * k + lane] = w;
+  }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+  __syncthreads();
+  const float4* po = reinterpret_cast<const float4*>(p.part_o + row * p.n_split * kD) + lane;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = warp; i < n; i += 4) {
+    const float w = weight[i];
+    const float4 x = po[(long long)i * 32];
     acc.x += w * x.x;
     acc.y += w * x.y;
     acc.z += w * x.z;
     acc.w += w * x.w;
   }
-  const float f = l == 0.f ? 0.f : 1.f / l;
-  const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+  sums[warp][lane] = acc;
+  __syncthreads();
+  const int c = threadIdx.x;
+  const float* sf = reinterpret_cast<const float*>(sums);
+  const float sum = (sf[c] + sf[kD + c]) + (sf[2 * kD + c] + sf[3 * kD + c]);
+  const float val = l == 0.f ? 0.f : sum / l;
   const int i = r / p.G, hq = kvh * p.G + r - i * p.G, Hq = p.Hkv * p.G;
-  const long long at = (((long long)b * p.Lq + i) * Hq + hq) * kD + 4 * lane;
-  acc.x = l == 0.f ? 0.f : acc.x * f;
-  acc.y = l == 0.f ? 0.f : acc.y * f;
-  acc.z = l == 0.f ? 0.f : acc.z * f;
-  acc.w = l == 0.f ? 0.f : acc.w * f;
-  uint2 v;
-  if (p.f16) {
-    v.x = as_u32(__floats2half2_rn(acc.x, acc.y));
-    v.y = as_u32(__floats2half2_rn(acc.z, acc.w));
-  } else {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(acc.x, acc.y), y = __floats2bfloat162_rn(acc.z, acc.w);
-    v.x = *reinterpret_cast<const uint32_t*>(&x);
-    v.y = *reinterpret_cast<const uint32_t*>(&y);
-  }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = v;
-  if (lane == 0) p.lse[((long long)b * Hq + hq) * p.Lq + i] = lse2 * 0.69314718055994531f;
+  const long long at = (((long long)b * p.Lq + i) * Hq + hq) * kD + c;
+  if (p.f16)
+    static_cast<__half*>(p.out)[at] = __float2half_rn(val);
+  else
+    static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(val);
+  if (c == 0)
+    p.lse[((long long)b * Hq + hq) * p.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-// Resident CTAs an SM that the split is planned for.
-constexpr int kResident = 2;
+// CTAs of attn_few_kernel that fit an SM: by shared memory (228 KB, 1 KB of it
+// the system's for each CTA) and by its launch bounds.
+template <int kBits, int kG>
+constexpr int resident_of(int nt) {
+  const int by_smem = 228 * 1024 / (int)(kWarps * Stage<kBits, kG>::kCount * Stage<kBits, kG>::kBytes + 2048);
+  const int by_regs = nt == 1 ? 4 : 2;
+  return by_smem < by_regs ? by_smem : by_regs;
+}
+int resident(int bits, int group, int nt) {
+  if (bits == 4)
+    return group == 32 ? resident_of<4, 4>(nt) : group == 64 ? resident_of<4, 2>(nt) : resident_of<4, 1>(nt);
+  return group == 32 ? resident_of<8, 4>(nt) : group == 64 ? resident_of<8, 2>(nt) : resident_of<8, 1>(nt);
+}
 
 struct Plan {
   bool many;
@@ -589,20 +612,20 @@ constexpr int kManyFrom = 33;
 
 // Parts of a sequence: the count that ends first when `units` x parts CTAs run
 // in waves, a part costing its tokens plus a fixed start and end.
-Plan plan(int B, int Hkv, long long rows, int max_len) {
+Plan plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
   Plan r;
   r.many = rows >= kManyFrom;
   r.nt = rows <= 8 ? 1 : 2;
   const int per_tile = r.many ? kManyRows : 8 * r.nt, tok = r.many ? kManyTok : kTok, least = r.many ? 1 : kWarps;
   r.n_rt = (int)((rows + per_tile - 1) / per_tile);
-  const long long units = (long long)B * Hkv * r.n_rt, slots = (long long)sm_count() * (r.many ? 1 : kResident);
+  const long long units = (long long)B * Hkv * r.n_rt, slots = (long long)sm_count() * (r.many ? 1 : resident(bits, group, r.nt));
   const int tiles = (max_len + tok - 1) / tok;
-  const double fixed = r.many ? 4 : 12, join = r.many ? 4 : 16;
+  const double fixed = r.many ? 4 : 12, join = r.many ? 4 : 8, each = r.many ? 0.2 : 0.1;
   double best = 0;
   r.n_split = 1;
-  for (int n = 1; n <= 256 && n * least <= (tiles > least ? tiles : least); ++n) {
+  for (int n = 1; n <= kMaxSplit && n * least <= (tiles > least ? tiles : least); ++n) {
     const long long waves = (units * n + slots - 1) / slots;
-    const double cost = (double)waves * ((tiles + n - 1) / n + fixed) + (n > 1 ? join : 0);
+    const double cost = (double)waves * ((tiles + n - 1) / n + fixed) + (n > 1 ? join + each * n : 0);
     if (n == 1 || cost < best) {
       best = cost;
       r.n_split = n;
@@ -617,7 +640,8 @@ cudaError_t launch_few(const AttnParams& p, long long blocks, cudaStream_t s) {
   constexpr uint32_t ring = kWarps * St::kCount * St::kBytes, join = kWarps * 8 * kNT * kD * 4;
   constexpr uint32_t smem = ring > join ? ring : join;
   auto kern = attn_few_kernel<kBits, kG, kNT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
   kern<<<(unsigned)blocks, kAttnThreads, smem, s>>>(p);
   return cudaGetLastError();
@@ -655,7 +679,7 @@ extern "C" size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, in
       cache->batch <= 0 || max_length < 0)
     return 0;
   const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
-  const kvq::Plan pl = kvq::plan(cache->batch, cache->n_kv_heads, rows, max_length);
+  const kvq::Plan pl = kvq::plan(cache->bits, cache->group, cache->batch, cache->n_kv_heads, rows, max_length);
   SizerOut z;
   float *a, *b;
   carve_parts(z, pl.n_split, rows * cache->batch * cache->n_kv_heads, &a, &b);
@@ -714,14 +738,14 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
   p.out = out;
   p.lse = lse;
   p.status = device_status();
-  const kvq::Plan pl = kvq::plan(p.B, p.Hkv, rows, max_length);
+  const kvq::Plan pl = kvq::plan(cache->bits, cache->group, p.B, p.Hkv, rows, max_length);
   p.n_rt = pl.n_rt;
   p.n_split = pl.n_split;
   Carver c(workspace, workspace_bytes);
   carve_parts(c, pl.n_split, rows * p.B * p.Hkv, &p.part_o, &p.part_lse);
   if (c.overflow) return set_error(CORE_ERR_WORKSPACE, f + ": workspace too small");
   const long long blocks = (long long)p.B * p.Hkv * pl.n_rt * pl.n_split;
-  const long long join_blocks = (rows * p.B * p.Hkv + 3) / 4;
+  const long long join_blocks = rows * p.B * p.Hkv;
   if (blocks > INT_MAX || join_blocks > INT_MAX)
     return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -2,6 +2,8 @@
 // arguments, the places of rows and tokens, and the join of a sequence's parts.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 #include "kvq_common.cuh"
 
@@ -81,6 +83,21 @@ __device__ __forceinline__ RowShift row_shift(float mx) {
 __device__ __forceinline__ float2 query_pair(uint32_t w, bool f16) {
   if (f16) return __half22float2(as_half2(w));
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Sets a kernel's shared memory limits at its first launch on a device: `done`
+// has a bit for each device that has them.
+inline cudaError_t prepare_kernel(const void* kern, uint32_t smem, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // The kernel for many query rows (attention_quant_many.cu): rows and tokens of a

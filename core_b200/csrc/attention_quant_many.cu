@@ -497,7 +497,8 @@ template <int kBits, int kG>
 cudaError_t launch_one(const AttnParams& p, long long blocks, cudaStream_t s) {
   constexpr uint32_t smem = ManySmem::kTotal + 1024;
   auto kern = attn_many_kernel<kBits, kG>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
   kern<<<(unsigned)blocks, kManyThreads, smem, s>>>(p);
   return cudaGetLastError();

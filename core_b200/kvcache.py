@@ -29,34 +29,39 @@ class QuantizedKV:
     """
 
     __slots__ = ("k_codes", "k_meta", "v_codes", "v_meta", "bits", "group", "batch", "n_kv_heads",
-                 "capacity", "device", "_struct", "_lengths", "max_length")
+                 "capacity", "index", "handle", "_lengths", "max_length")
 
     def __init__(self, k_codes: torch.Tensor, k_meta: torch.Tensor, v_codes: torch.Tensor,
                  v_meta: torch.Tensor):
         """Wraps existing buffers (their rows are the caller's; lengths start at 0)."""
-        if k_codes.dim() != 4 or k_meta.dim() != 5:
+        shape, meta_shape = k_codes.shape, k_meta.shape
+        if len(shape) != 4 or len(meta_shape) != 5:
             raise ValueError("codes must be (B, Hkv, capacity, 16 * bits), meta "
                              "(B, Hkv, capacity, 128 / group, 2)")
-        B, H, cap, width = k_codes.shape
-        groups = k_meta.shape[3]
+        B, H, cap, width = shape
+        groups = meta_shape[3]
         if width not in (64, 128) or groups not in (1, 2, 4):
             raise ValueError("a row takes 64 (4 bits) or 128 (8 bits) bytes and 1, 2 or 4 groups")
-        if cap <= 0 or cap % CAPACITY_STEP:
+        if B <= 0 or H <= 0 or cap <= 0 or cap % CAPACITY_STEP:
             raise ValueError(f"capacity must be a positive multiple of {CAPACITY_STEP}")
-        for codes, meta in ((k_codes, k_meta), (v_codes, v_meta)):
-            if codes.shape != k_codes.shape or codes.dtype != torch.uint8 or not codes.is_contiguous():
-                raise ValueError("codes must be contiguous uint8 tensors of one shape")
-            if (meta.shape != (B, H, cap, groups, 2) or meta.dtype != torch.float16
-                    or not meta.is_contiguous()):
-                raise ValueError("meta must be contiguous float16 tensors (B, Hkv, capacity, groups, 2)")
-            if not codes.is_cuda or codes.device != k_codes.device or meta.device != k_codes.device:
-                raise ValueError("core_b200 operates on CUDA tensors only, all on one device")
+        at = k_codes.get_device()
+        if at < 0 or k_meta.get_device() != at or v_codes.get_device() != at or v_meta.get_device() != at:
+            raise ValueError("core_b200 operates on CUDA tensors only, all on one device")
+        if (v_codes.shape != shape or k_codes.dtype is not torch.uint8 or v_codes.dtype is not torch.uint8
+                or not k_codes.is_contiguous() or not v_codes.is_contiguous()):
+            raise ValueError("codes must be contiguous uint8 tensors of one shape")
+        if (meta_shape != (B, H, cap, groups, 2) or v_meta.shape != meta_shape
+                or k_meta.dtype is not torch.float16 or v_meta.dtype is not torch.float16
+                or not k_meta.is_contiguous() or not v_meta.is_contiguous()):
+            raise ValueError("meta must be contiguous float16 tensors (B, Hkv, capacity, groups, 2)")
         self.k_codes, self.k_meta, self.v_codes, self.v_meta = k_codes, k_meta, v_codes, v_meta
         self.bits, self.group = width // 16, 128 // groups
         self.batch, self.n_kv_heads, self.capacity = B, H, cap
-        self.device = k_codes.device
-        self._struct = _lib.CoreKvq(k_codes.data_ptr(), k_meta.data_ptr(), v_codes.data_ptr(),
-                                    v_meta.data_ptr(), B, H, cap, self.bits, self.group)
+        self.index = at
+        # the core_kvq_t that the C-ABI takes
+        self.handle = ctypes.byref(_lib.CoreKvq(
+            k_codes.data_ptr(), k_meta.data_ptr(), v_codes.data_ptr(), v_meta.data_ptr(), B, H, cap,
+            self.bits, self.group))
         self._lengths = None
         self.max_length = 0
 
@@ -83,9 +88,8 @@ class QuantizedKV:
         return self._lengths
 
     @property
-    def handle(self):
-        """The ``core_kvq_t`` pointer the C-ABI takes."""
-        return ctypes.byref(self._struct)
+    def device(self) -> torch.device:
+        return self.k_codes.device
 
     @property
     def nbytes(self) -> int:

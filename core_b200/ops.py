@@ -165,33 +165,47 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
 # ---------------------------------------------------------------------------
 
 _KVQ_DTYPES = _READOUT_DTYPES
+_I64X3 = ctypes.c_int64 * 3
+
+# One token is written, read or attended to in a few microseconds: these wrappers
+# check in as few calls as they can.
 
 
-def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """t itself where its last dim is contiguous and its base and other strides
-    are 16-byte aligned, else a contiguous copy."""
-    size = t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:-1]):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _on_device(t: torch.Tensor, cache, name: str) -> None:
+    if t.get_device() != cache.index:
+        if not t.is_cuda:
+            raise ValueError("core_b200 operates on CUDA tensors only (no CPU path)")
+        raise ValueError(f"{name} must be on the cache's device")
+
+
+def _aligned_rows(t: torch.Tensor):
+    """(t, its outer strides) where t's last dim is contiguous and its base and
+    other strides are 16-byte aligned, else those of a contiguous copy."""
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or t.data_ptr() % 16 or (s0 | s1 | s2) * t.element_size() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, s2, _ = t.stride()
+    return t, _I64X3(s0, s1, s2)
 
 
 def _per_sequence(value, cache, name: str):
     """(pointer to (B,) int32 on the device, scalar) of an int or a tensor."""
     if not isinstance(value, torch.Tensor):
         return None, int(value)
-    if value.shape != (cache.batch,) or value.dtype != torch.int32 or not value.is_contiguous():
+    if value.shape != (cache.batch,) or value.dtype is not torch.int32 or not value.is_contiguous():
         raise ValueError(f"{name} must be an int or a contiguous (B,) int32 tensor")
-    if value.device != cache.device:
-        raise ValueError(f"{name} must be on the cache's device")
+    _on_device(value, cache, name)
     return value.data_ptr(), 0
 
 
 def _row_index(index, cache, name: str):
     if index.dim() != 2 or index.shape[0] != cache.batch:
         raise ValueError(f"{name} must be (B, n)")
-    if index.device != cache.device:
-        raise ValueError(f"{name} must be on the cache's device")
+    _on_device(index, cache, name)
     return index.to(torch.int32).contiguous()
 
 
@@ -206,29 +220,32 @@ def kv_quantize(keys: torch.Tensor, values: torch.Tensor, cache, start, *,
     only the first counts[b] rows.  Slots or source rows out of range are
     skipped and reported by :func:`status`.
     """
-    _require_cuda(keys, values, index, counts)
+    _on_device(keys, cache, "keys")
+    _on_device(values, cache, "values")
     code = _KVQ_DTYPES.get(keys.dtype)
-    if code is None or values.dtype != keys.dtype:
+    if code is None or values.dtype is not keys.dtype:
         raise TypeError("kv_quantize takes keys and values of one dtype, bf16, f16 or f32")
-    if (keys.dim() != 4 or keys.shape != values.shape or keys.shape[0] != cache.batch
-            or keys.shape[1] != cache.n_kv_heads or keys.shape[3] != HEAD_DIM):
+    shape = keys.shape
+    if (len(shape) != 4 or shape != values.shape or shape[0] != cache.batch
+            or shape[1] != cache.n_kv_heads or shape[3] != HEAD_DIM):
         raise ValueError(f"keys and values must be ({cache.batch}, {cache.n_kv_heads}, L, {HEAD_DIM})")
-    if keys.device != cache.device or values.device != cache.device:
-        raise ValueError("keys and values must be on the cache's device")
-    keys, values = _aligned_rows(keys), _aligned_rows(values)
-    n = L = keys.shape[2]
+    keys, ks = _aligned_rows(keys)
+    values, vs = _aligned_rows(values)
+    n = L = shape[2]
     if index is not None:
         index = _row_index(index, cache, "index")
         n = index.shape[1]
     if n == 0:
         return
     at, at0 = _per_sequence(start, cache, "start")
-    cnt = None if counts is None else _per_sequence(counts, cache, "counts")[0]
-    ks, vs = keys.stride(), values.stride()
+    cnt = None
+    if counts is not None:
+        if not isinstance(counts, torch.Tensor):
+            raise ValueError("counts must be a contiguous (B,) int32 tensor")
+        cnt = _per_sequence(counts, cache, "counts")[0]
     check(_lib.load().core_kvq_quantize(
-        cache.handle, code, keys.data_ptr(), (ctypes.c_int64 * 3)(*ks[:3]), values.data_ptr(),
-        (ctypes.c_int64 * 3)(*vs[:3]), L, n, None if index is None else index.data_ptr(), at, at0,
-        cnt, _stream(cache.device)))
+        cache.handle, code, keys.data_ptr(), ks, values.data_ptr(), vs, L, n,
+        None if index is None else index.data_ptr(), at, at0, cnt, _raw_stream(cache.index)))
 
 
 def kv_dequantize(cache, *, start=0, count: int | None = None, index: torch.Tensor | None = None,
@@ -239,23 +256,20 @@ def kv_dequantize(cache, *, start=0, count: int | None = None, index: torch.Tens
     code = _KVQ_DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"kv_dequantize gives bf16, f16 or f32; got {dtype}")
-    _require_cuda(index)
-    at, at0 = None, 0
+    at, at0, idx = None, 0, None
     if index is not None:
         index = _row_index(index, cache, "index")
-        n = index.shape[1]
+        n, idx = index.shape[1], index.data_ptr()
     else:
         if count is None or count < 0:
             raise ValueError("kv_dequantize needs index, or a count of slots")
         n = int(count)
         at, at0 = _per_sequence(start, cache, "start")
-    shape = (cache.batch, cache.n_kv_heads, n, HEAD_DIM)
-    k = torch.empty(shape, dtype=dtype, device=cache.device)
-    v = torch.empty(shape, dtype=dtype, device=cache.device)
+    k = cache.k_meta.new_empty((cache.batch, cache.n_kv_heads, n, HEAD_DIM), dtype=dtype)
+    v = torch.empty_like(k)
     if n:
-        check(_lib.load().core_kvq_dequantize(
-            cache.handle, code, n, None if index is None else index.data_ptr(), at, at0,
-            k.data_ptr(), v.data_ptr(), _stream(cache.device)))
+        check(_lib.load().core_kvq_dequantize(cache.handle, code, n, idx, at, at0, k.data_ptr(),
+                                              v.data_ptr(), _raw_stream(cache.index)))
     return k, v
 
 
@@ -273,16 +287,15 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     Returns (out (B, Lq, Hq, 128) in q's dtype, lse (B, Hq, Lq) f32); a row that
     sees no token gives 0 and -inf.
     """
-    _require_cuda(q, key_mask)
-    code = _ATTN_DTYPES.get(q.dtype)
+    _on_device(q, cache, "q")
+    dtype = q.dtype
+    code = _ATTN_DTYPES.get(dtype)
     if code is None:
-        raise TypeError(f"attention_quantized takes bf16 or f16 queries; got {q.dtype}")
+        raise TypeError(f"attention_quantized takes bf16 or f16 queries; got {dtype}")
     if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != HEAD_DIM or q.shape[1] % cache.n_kv_heads:
         raise ValueError(f"q must be ({cache.batch}, Hq, Lq, {HEAD_DIM}) with Hq a multiple of "
                          f"{cache.n_kv_heads}")
-    if q.device != cache.device:
-        raise ValueError("q must be on the cache's device")
-    q = _aligned_rows(q)
+    q, strides = _aligned_rows(q)
     B, Hq, Lq, _ = q.shape
     at, n = _per_sequence(lengths, cache, "lengths")
     if at is not None:
@@ -292,27 +305,27 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
         if (key_mask.dim() != 2 or key_mask.shape[0] != B or key_mask.shape[1] < n
                 or key_mask.dtype not in (torch.bool, torch.uint8)):
             raise ValueError("key_mask must be a (B, >= max_length) bool or uint8 tensor")
-        if key_mask.device != cache.device:
-            raise ValueError("key_mask must be on the cache's device")
+        _on_device(key_mask, cache, "key_mask")
         if key_mask.stride(1) != 1 or (B > 1 and key_mask.stride(0) < key_mask.shape[1]):
             key_mask = key_mask.contiguous()
         mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if B > 1 else key_mask.shape[1]
     if out is None:
-        out = torch.empty((B, Lq, Hq, HEAD_DIM), dtype=q.dtype, device=q.device)
-    elif out.shape != (B, Lq, Hq, HEAD_DIM) or not out.is_contiguous() or out.dtype != q.dtype:
-        raise ValueError("out must be a contiguous (B, Lq, Hq, 128) tensor of q's dtype")
-    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
+        out = q.new_empty((B, Lq, Hq, HEAD_DIM))
+    else:
+        if out.shape != (B, Lq, Hq, HEAD_DIM) or not out.is_contiguous() or out.dtype is not dtype:
+            raise ValueError("out must be a contiguous (B, Lq, Hq, 128) tensor of q's dtype")
+        _on_device(out, cache, "out")
+    lse = q.new_empty((B, Hq, Lq), dtype=torch.float32)
     if Lq == 0:
         return out, lse
     lib = _lib.load()
     need = lib.core_kvq_attention_workspace_bytes(cache.handle, Hq, Lq, n)
-    ws = _workspace(need, q.device) if need else None
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
-    st = q.stride()
     check(lib.core_kvq_attention(
-        cache.handle, code, Hq, Lq, q.data_ptr(), (ctypes.c_int64 * 3)(*st[:3]), at, n, mask,
-        mask_stride, 1 if causal else 0, scale, out.data_ptr(), lse.data_ptr(),
-        None if ws is None else ws.data_ptr(), need, _stream(q.device)))
+        cache.handle, code, Hq, Lq, q.data_ptr(), strides, at, n, mask, mask_stride,
+        1 if causal else 0, scale, out.data_ptr(), lse.data_ptr(),
+        None if ws is None else ws.data_ptr(), need, _raw_stream(cache.index)))
     return out, lse
 
 
