@@ -100,165 +100,234 @@ __device__ __forceinline__ void Piece<__half>::get(float (&x)[8]) const {
   }
 }
 
-struct Grid {  // a group's scale and zero, and what the codes are computed with
+// A group's scale and zero (the word of both as it is stored), and what its
+// codes are computed with.
+struct Grid {
   float z, inv;
   uint32_t word;
+  bool plain;  // none of the group's channels needs a clamp
 };
 
 template <int kBits>
-__device__ __forceinline__ Grid make_grid(float lo, float hi) {
-  constexpr float c = kBits == 4 ? 1.0f / 15.0f : 1.0f / 255.0f;
+__device__ __forceinline__ Grid grid_of(float lo, float hi) {
+  constexpr float c = kBits == 4 ? 1.0f / 15.0f : 1.0f / 255.0f, top = kBits == 4 ? 15.f : 255.f;
+  const float lo0 = lo, hi0 = hi;
   lo = max_nan(min_nan(lo, kLimit), -kLimit);
   hi = max_nan(min_nan(hi, kLimit), -kLimit);
-  const __half z = __float2half_rn(lo), s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), c));
+  const __half2 sz = __floats2half2_rn(__fmul_rn(__fsub_rn(hi, lo), c), lo);
+  const float2 f = __half22float2(sz);
   Grid g;
-  g.z = __half2float(z);
-  const float sf = __half2float(s);
-  g.inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
-  g.word = (uint32_t)__half_as_ushort(s) | ((uint32_t)__half_as_ushort(z) << 16);
+  g.z = f.y;
+  g.inv = f.x > 0.f ? __frcp_rn(f.x) : 0.f;
+  g.word = as_u32(sz);
+  // the extrema fall on codes 0 .. N, and neither was saturated (NaN: false)
+  const float first = __fmul_rn(__fsub_rn(lo, g.z), g.inv), last = __fmul_rn(__fsub_rn(hi, g.z), g.inv);
+  g.plain = lo == lo0 && hi == hi0 && first >= -0.5f && last < top + 0.5f;
   return g;
 }
 
-// Codes of eight channels: one word (4 bits) or two (8 bits).  The extrema were
-// saturated and the channels were not: a channel beyond the limit lands on the
-// first or last code all the same, as the saturated one does, unless the whole
-// group is (the saturated scale is then zero or tiny), so channels are clamped
-// where an extremum was.
+// Eight codes of kBits each from floats 1.5 2^23 + n: the integer lies in the low
+// bits, so shifted sums of the bit patterns give the word once the patterns of
+// 1.5 2^23 are taken off again (modulo 2^32).
 template <int kBits>
-__device__ __forceinline__ void encode(const float (&x)[8], const Grid& g, bool clamp, uint32_t (&w)[kBits / 4]) {
+__device__ __forceinline__ void pack_codes(const float (&r)[8], uint32_t* w) {
+  constexpr uint32_t m = 0x4B400000u;  // the bits of 1.5 2^23
+  if constexpr (kBits == 4) {
+    constexpr int at[8] = {0, 16, 4, 20, 8, 24, 12, 28};
+    constexpr uint32_t off = m + (m << 4) + (m << 8) + (m << 12) + (m << 16) + (m << 20) + (m << 24) + (m << 28);
+    uint32_t x = 0u - off;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x += __float_as_uint(r[i]) << at[i];
+    w[0] = x;
+  } else {
+    constexpr int at[4] = {0, 16, 8, 24};
+    constexpr uint32_t off = m + (m << 8) + (m << 16) + (m << 24);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t x = 0u - off;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x += __float_as_uint(r[4 * h + i]) << at[i];
+      w[h] = x;
+    }
+  }
+}
+
+// Codes of eight channels: one word (4 bits) or two (8 bits).
+template <int kBits>
+__device__ __forceinline__ void encode(const float (&x)[8], const Grid& g, uint32_t* w) {
   constexpr float top = kBits == 4 ? 15.f : 255.f;
-  uint32_t n[8];
+  constexpr float magic = 12582912.f;  // 1.5 2^23: adding it rounds to the nearest integer, ties to even
+  float r[8];
+  if (g.plain) {
+    const unsigned long long nz = f2_pack(-g.z, -g.z), mg = f2_pack(magic, magic);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float v = x[i];
-    if (clamp) v = fmaxf(fminf(v, kLimit), -kLimit);
-    const float y = fminf(fmaxf(__fmul_rn(__fsub_rn(v, g.z), g.inv), 0.f), top);
-    // adding 1.5 2^23 rounds to the nearest integer (ties to even) in the low bits
-    n[i] = __float_as_uint(__fadd_rn(y, 12582912.f)) & (kBits == 4 ? 15u : 255u);
-  }
-  if constexpr (kBits == 4) {
-    w[0] = n[0] | n[2] << 4 | n[4] << 8 | n[6] << 12 | n[1] << 16 | n[3] << 20 | n[5] << 24 | n[7] << 28;
+    for (int i = 0; i < 8; i += 2) {
+      // the product is one scalar multiplication a channel: the assembler joins a
+      // packed one with the addition into an fma, whose single rounding moves ties
+      const unsigned long long d = f2_add(f2_pack(x[i], x[i + 1]), nz);
+      const unsigned long long y = f2_add(f2_pack(__fmul_rn(f2_lo(d), g.inv), __fmul_rn(f2_hi(d), g.inv)), mg);
+      r[i] = f2_lo(y);
+      r[i + 1] = f2_hi(y);
+    }
   } else {
-    w[0] = n[0] | n[2] << 8 | n[1] << 16 | n[3] << 24;
-    w[1] = n[4] | n[6] << 8 | n[5] << 16 | n[7] << 24;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = fmaxf(fminf(x[i], kLimit), -kLimit);  // NaN: any code, its scale is NaN
+      r[i] = __fadd_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(v, g.z), g.inv), 0.f), top), magic);
+    }
   }
+  pack_codes<kBits>(r, w);
 }
 
-// kSteps-lane extrema of a group whose lanes differ in the given lane bits.
-__device__ __forceinline__ void reduce(float& lo, float& hi, int bit) {
-  lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, bit));
-  hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, bit));
-}
-__device__ __forceinline__ void extrema(const float (&x)[8], float& lo, float& hi) {
-  lo = hi = x[0];
+// Extrema of 16 channels (or of 8), as a (least, greatest) pair that NaN passes
+// through: f32, or both as the halves of one register, which the shuffles then
+// move at once.
+template <typename T>
+struct Extrema;
+template <>
+struct Extrema<float> {
+  float lo, hi;
+  __device__ __forceinline__ void of(const Piece<float>& p) {
+    float x[8];
+    p.get(x);
+    lo = hi = x[0];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
+    for (int i = 1; i < 8; ++i) {
+      lo = min_nan(lo, x[i]);
+      hi = max_nan(hi, x[i]);
+    }
   }
+  __device__ __forceinline__ void with(const Extrema& o) {
+    lo = min_nan(lo, o.lo);
+    hi = max_nan(hi, o.hi);
+  }
+  __device__ __forceinline__ void close() {}
+  __device__ __forceinline__ void across(int bit) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, bit));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, bit));
+  }
+  __device__ __forceinline__ float least() const { return lo; }
+  __device__ __forceinline__ float greatest() const { return hi; }
+};
+template <typename T2>
+__device__ __forceinline__ T2 pair_of(uint32_t u) {
+  return *reinterpret_cast<T2*>(&u);
 }
-
-template <int kBits, int kG>
-__device__ __forceinline__ void write_row(const float (&p0)[8], const float (&p1)[8], bool keys, int m,
-                                          uint32_t tok, bool live, uint8_t* codes, uint32_t* meta) {
-  // K: lane m = 4 a + t holds channels 64 a + 8 t and 64 a + 32 + 8 t;
-  // V: channels 16 m and 16 m + 8
-  float lo0, hi0, lo1, hi1;
-  extrema(p0, lo0, hi0);
-  extrema(p1, lo1, hi1);
-  if (!(keys && kG == 4)) {  // both pieces in one group
-    lo0 = min_nan(lo0, lo1);
-    hi0 = max_nan(hi0, hi1);
+template <typename T, typename T2>
+struct Extrema16 {
+  T2 lo, hi;  // of even and odd channels; after close(): lo = (least, -greatest)
+  __device__ __forceinline__ void of(const Piece<T>& p) {
+    const uint32_t u[4] = {p.v[0].x, p.v[0].y, p.v[0].z, p.v[0].w};
+    lo = hi = pair_of<T2>(u[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      lo = __hmin2_nan(lo, pair_of<T2>(u[i]));
+      hi = __hmax2_nan(hi, pair_of<T2>(u[i]));
+    }
   }
-  reduce(lo0, hi0, 1);
-  if (keys || kG <= 2) reduce(lo0, hi0, 2);
-  if (kG == 1) reduce(lo0, hi0, 4);
-  if (keys && kG == 4) {
-    reduce(lo1, hi1, 1);
-    reduce(lo1, hi1, 2);
-  } else {
-    lo1 = lo0;
-    hi1 = hi0;
+  __device__ __forceinline__ void with(const Extrema16& o) {
+    lo = __hmin2_nan(lo, o.lo);
+    hi = __hmax2_nan(hi, o.hi);
   }
-  const Grid g0 = make_grid<kBits>(lo0, hi0);
-  const Grid g1 = keys && kG == 4 ? make_grid<kBits>(lo1, hi1) : g0;
-  const bool c0 = !(fabsf(lo0) <= kLimit && fabsf(hi0) <= kLimit);
-  const bool c1 = !(fabsf(lo1) <= kLimit && fabsf(hi1) <= kLimit);
-  uint32_t w0[kBits / 4], w1[kBits / 4];
-  encode<kBits>(p0, g0, c0, w0);
-  encode<kBits>(p1, g1, c1, w1);
-  if (!live) return;
-  const int a = m >> 2, t = m & 3;
-  if constexpr (kBits == 4) {
-    const uint32_t at = keys ? 16u * t + 8u * a : (8u * m) ^ value_swizzle<4>(tok);
-    *reinterpret_cast<uint2*>(codes + at) = make_uint2(w0[0], w1[0]);
-  } else {
-    const uint32_t at = (16u * m) ^ (keys ? key_swizzle<8>(tok) : value_swizzle<8>(tok));
-    *reinterpret_cast<uint4*>(codes + at) = make_uint4(w0[0], w0[1], w1[0], w1[1]);
+  __device__ __forceinline__ void close() {
+    const T2 n = __hneg2(hi);
+    // (lo.x, -hi.x) and (lo.y, -hi.y): one minimum leaves (least, -greatest)
+    lo = __hmin2_nan(__halves2(__low2(lo), __low2(n)), __halves2(__high2(lo), __high2(n)));
   }
-  if (keys) {
-    if (kG == 4 && t == 0) *reinterpret_cast<uint2*>(meta + 2 * a) = make_uint2(g0.word, g1.word);
-    if (kG == 2 && t == 0) meta[a] = g0.word;
-  } else {
-    if (kG == 4 && (m & 1) == 0) meta[m >> 1] = g0.word;
-    if (kG == 2 && t == 0) meta[a] = g0.word;
+  __device__ __forceinline__ void across(int bit) { lo = __hmin2_nan(lo, __shfl_xor_sync(0xffffffffu, lo, bit)); }
+  __device__ __forceinline__ float least() const { return to_float(__low2(lo)); }
+  __device__ __forceinline__ float greatest() const { return -to_float(__high2(lo)); }
+  static __device__ __forceinline__ __half2 __halves2(__half a, __half b) { return __halves2half2(a, b); }
+  static __device__ __forceinline__ __nv_bfloat162 __halves2(__nv_bfloat16 a, __nv_bfloat16 b) {
+    return __halves2bfloat162(a, b);
   }
-  if (kG == 1 && m == 0) meta[0] = g0.word;
-}
+  static __device__ __forceinline__ __half __low2(__half2 a) { return __low2half(a); }
+  static __device__ __forceinline__ __half __high2(__half2 a) { return __high2half(a); }
+  static __device__ __forceinline__ __nv_bfloat16 __low2(__nv_bfloat162 a) { return __low2bfloat16(a); }
+  static __device__ __forceinline__ __nv_bfloat16 __high2(__nv_bfloat162 a) { return __high2bfloat16(a); }
+  static __device__ __forceinline__ float to_float(__half a) { return __half2float(a); }
+  static __device__ __forceinline__ float to_float(__nv_bfloat16 a) { return __bfloat162float(a); }
+};
+template <>
+struct Extrema<__half> : Extrema16<__half, __half2> {};
+template <>
+struct Extrema<__nv_bfloat16> : Extrema16<__nv_bfloat16, __nv_bfloat162> {};
 
 constexpr int kThreads = 256;
+constexpr int kRows = kThreads / 8;  // rows of a block: eight lanes each
+
+// Lane m of a row's eight holds channels 16 m .. 16 m + 15.
+template <typename T, int kBits, int kG>
+__device__ __forceinline__ void write_row(const Piece<T>& p0, const Piece<T>& p1, bool keys, int m, uint32_t tok,
+                                          bool live, uint8_t* codes, uint32_t* meta) {
+  Extrema<T> e, e1;
+  e.of(p0);
+  e1.of(p1);
+  e.with(e1);
+  e.close();
+  e.across(1);
+  if (kG <= 2) e.across(2);
+  if (kG == 1) e.across(4);
+  const Grid g = grid_of<kBits>(e.least(), e.greatest());
+  uint32_t w[kBits / 2];
+  float x[8];
+  p0.get(x);
+  encode<kBits>(x, g, w);
+  p1.get(x);
+  encode<kBits>(x, g, w + kBits / 4);
+  if (!live) return;
+  if (keys) {
+    // channels 32 b + 8 t .. with b = m / 2 and t = 2 (m & 1), then t + 1
+    if constexpr (kBits == 4) {
+      uint32_t* to = reinterpret_cast<uint32_t*>(codes) + 8 * (m & 1) + (m >> 1);
+      to[0] = w[0];
+      to[4] = w[1];
+    } else {
+      const uint32_t at = (64u * (m >> 2) + 32u * (m & 1) + 8u * ((m >> 1) & 1)) ^ key_swizzle<8>(tok);
+      *reinterpret_cast<uint2*>(codes + at) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(codes + at + 16) = make_uint2(w[2], w[3]);
+    }
+  } else {
+    if constexpr (kBits == 4)
+      *reinterpret_cast<uint2*>(codes + ((8u * m) ^ value_swizzle<4>(tok))) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint4*>(codes + ((16u * m) ^ value_swizzle<8>(tok))) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if ((m & (8 / kG - 1)) == 0) meta[m / (8 / kG)] = g.word;
+}
 
 template <typename T, int kBits, int kG>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const WriteParams p) {
-  const long long total = (long long)p.c.B * p.c.H * p.T;
   const int m = threadIdx.x & 7;
-  const long long step = (long long)gridDim.x * (kThreads / 8);
+  const unsigned chunks = ((unsigned)p.T + kRows - 1) / kRows, units = (unsigned)(p.c.B * p.c.H) * chunks;
   // whole warps stay in the loop: the shuffles need every lane of a row
-  for (long long r0 = (long long)blockIdx.x * (kThreads / 8); r0 < total; r0 += step) {
-    const long long r = r0 + (threadIdx.x >> 3);
-    bool live = r < total;
-    int bh = 0, t = 0;
-    if (live) {
-      if (total <= UINT_MAX) {
-        bh = (int)((unsigned)r / (unsigned)p.T);
-        t = (int)((unsigned)r - (unsigned)bh * (unsigned)p.T);
-      } else {
-        bh = (int)(r / p.T);
-        t = (int)(r - (long long)bh * p.T);
-      }
-    }
+  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+    const int bh = (int)(u / chunks), t = (int)(u - (unsigned)bh * chunks) * kRows + (int)(threadIdx.x >> 3);
     const int b = bh / p.c.H, h = bh - b * p.c.H;
-    if (live && p.counts != nullptr) live = t < p.counts[b];
-    long long slot = 0;
+    int n = p.T;
+    if (p.counts != nullptr) n = min(n, p.counts[b]);
+    bool live = t < n;
+    const long long slot = (long long)(p.start != nullptr ? p.start[b] : p.start0) + t;
     int src = t;
-    if (live) {
-      slot = (long long)(p.start != nullptr ? p.start[b] : p.start0) + t;
-      if (p.index != nullptr) src = p.index[(long long)b * p.T + t];
-      if (slot < 0 || slot >= p.c.cap || src < 0 || src >= p.L) {
-        if (m == 0) record_error(p.status, CORE_ERR_INVALID_ARG, slot < 0 || slot >= p.c.cap ? 1401 : 1402, t);
-        live = false;
-      }
+    if (live && p.index != nullptr) src = p.index[(long long)b * p.T + t];
+    if (live && (slot < 0 || slot >= p.c.cap || src < 0 || src >= p.L)) {
+      if (m == 0) record_error(p.status, CORE_ERR_INVALID_ARG, slot < 0 || slot >= p.c.cap ? 1401 : 1402, t);
+      live = false;
     }
-    Piece<T> k0, k1, v0, v1;
+    Piece<T> k0{}, k1{}, v0{}, v1{};
     if (live) {
-      const T* k = static_cast<const T*>(p.src[0]) + b * p.sb[0] + h * p.sh[0] + src * p.sl[0];
-      const T* v = static_cast<const T*>(p.src[1]) + b * p.sb[1] + h * p.sh[1] + src * p.sl[1];
-      const int at = 64 * (m >> 2) + 8 * (m & 3);
-      k0.load(k + at);
-      k1.load(k + at + 32);
-      v0.load(v + 16 * m);
-      v1.load(v + 16 * m + 8);
-    } else {
-      k0 = k1 = v0 = v1 = Piece<T>{};
+      const T* k = static_cast<const T*>(p.src[0]) + b * p.sb[0] + h * p.sh[0] + src * p.sl[0] + 16 * m;
+      const T* v = static_cast<const T*>(p.src[1]) + b * p.sb[1] + h * p.sh[1] + src * p.sl[1] + 16 * m;
+      k0.load(k);
+      k1.load(k + 8);
+      v0.load(v);
+      v1.load(v + 8);
     }
     const long long row = (long long)bh * p.c.cap + slot;
-    float x[8], y[8];
-    k0.get(x);
-    k1.get(y);
-    write_row<kBits, kG>(x, y, true, m, (uint32_t)slot, live, p.c.codes[0] + row * (16 * kBits), p.c.meta[0] + row * kG);
-    v0.get(x);
-    v1.get(y);
-    write_row<kBits, kG>(x, y, false, m, (uint32_t)slot, live, p.c.codes[1] + row * (16 * kBits), p.c.meta[1] + row * kG);
+    write_row<T, kBits, kG>(k0, k1, true, m, (uint32_t)slot, live, p.c.codes[0] + row * (16 * kBits),
+                            p.c.meta[0] + row * kG);
+    write_row<T, kBits, kG>(v0, v1, false, m, (uint32_t)slot, live, p.c.codes[1] + row * (16 * kBits),
+                            p.c.meta[1] + row * kG);
   }
 }
 
@@ -298,34 +367,28 @@ __device__ __forceinline__ void decode_store(const uint32_t* w, uint32_t meta, T
 
 template <typename T, int kBits, int kG>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const ReadParams p) {
-  const long long total = (long long)p.c.B * p.c.H * p.T;
   const int m = threadIdx.x & 7, a = m >> 2, q = m & 3;
-  const long long step = (long long)gridDim.x * (kThreads / 8);
-  for (long long r = (long long)blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3); r < total; r += step) {
-    int bh, t;
-    if (total <= UINT_MAX) {
-      bh = (int)((unsigned)r / (unsigned)p.T);
-      t = (int)((unsigned)r - (unsigned)bh * (unsigned)p.T);
-    } else {
-      bh = (int)(r / p.T);
-      t = (int)(r - (long long)bh * p.T);
-    }
+  const unsigned chunks = ((unsigned)p.T + kRows - 1) / kRows, units = (unsigned)(p.c.B * p.c.H) * chunks;
+  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+    const int bh = (int)(u / chunks), t = (int)(u - (unsigned)bh * chunks) * kRows + (int)(threadIdx.x >> 3);
+    if (t >= p.T) continue;
     const int b = bh / p.c.H;
     long long slot;
     if (p.index != nullptr)
       slot = p.index[(long long)b * p.T + t];
     else
       slot = (long long)(p.start != nullptr ? p.start[b] : p.start0) + t;
-    T* ok = static_cast<T*>(p.dst[0]) + r * kD;
-    T* ov = static_cast<T*>(p.dst[1]) + r * kD;
-    const int at = 64 * a + 8 * q;
+    const long long to = ((long long)bh * p.T + t) * kD;
+    // K: lane m = 4 a + q decodes channels 64 a + 8 q and 64 a + 32 + 8 q; V: 16 m
+    T* ok = static_cast<T*>(p.dst[0]) + to + 64 * a + 8 * q;
+    T* ov = static_cast<T*>(p.dst[1]) + to + 16 * m;
     if (slot < 0 || slot >= p.c.cap) {
       if (m == 0) record_error(p.status, CORE_ERR_INVALID_ARG, 1411, t);
       const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      store8(ok + at, zero);
-      store8(ok + at + 32, zero);
-      store8(ov + 16 * m, zero);
-      store8(ov + 16 * m + 8, zero);
+      store8(ok, zero);
+      store8(ok + 32, zero);
+      store8(ov, zero);
+      store8(ov + 8, zero);
       continue;
     }
     const long long row = (long long)bh * p.c.cap + slot;
@@ -337,28 +400,20 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const ReadParams p
     if constexpr (kBits == 4) {
       const uint2 x = *reinterpret_cast<const uint2*>(kc + 16 * q + 8 * a);
       const uint2 y = *reinterpret_cast<const uint2*>(vc + ((8u * m) ^ value_swizzle<4>((uint32_t)slot)));
-      kw[0] = x.x;
-      kw[1] = x.y;
-      vw[0] = y.x;
-      vw[1] = y.y;
+      kw[0] = x.x; kw[1] = x.y;
+      vw[0] = y.x; vw[1] = y.y;
     } else {
       const uint4 x = *reinterpret_cast<const uint4*>(kc + ((16u * m) ^ key_swizzle<8>((uint32_t)slot)));
       const uint4 y = *reinterpret_cast<const uint4*>(vc + ((16u * m) ^ value_swizzle<8>((uint32_t)slot)));
-      kw[0] = x.x;
-      kw[1] = x.y;
-      kw[2] = x.z;
-      kw[3] = x.w;
-      vw[0] = y.x;
-      vw[1] = y.y;
-      vw[2] = y.z;
-      vw[3] = y.w;
+      kw[0] = x.x; kw[1] = x.y; kw[2] = x.z; kw[3] = x.w;
+      vw[0] = y.x; vw[1] = y.y; vw[2] = y.z; vw[3] = y.w;
     }
     const uint32_t k0 = km[kG == 4 ? 2 * a : kG == 2 ? a : 0], k1 = kG == 4 ? km[2 * a + 1] : k0;
     const uint32_t v0 = vm[kG == 4 ? m >> 1 : kG == 2 ? a : 0];
-    decode_store<T, kBits>(kw, k0, ok + at);
-    decode_store<T, kBits>(kw + kBits / 4, k1, ok + at + 32);
-    decode_store<T, kBits>(vw, v0, ov + 16 * m);
-    decode_store<T, kBits>(vw + kBits / 4, v0, ov + 16 * m + 8);
+    decode_store<T, kBits>(kw, k0, ok);
+    decode_store<T, kBits>(kw + kBits / 4, k1, ok + 32);
+    decode_store<T, kBits>(vw, v0, ov);
+    decode_store<T, kBits>(vw + kBits / 4, v0, ov + 8);
   }
 }
 
@@ -400,10 +455,9 @@ kvq::Cache device_cache(const core_kvq_t* c) {
   return d;
 }
 
-// Eight lanes a row, at most 8 resident blocks' worth of grid per SM.
-int row_blocks(long long rows) {
-  const long long need = (rows + kvq::kThreads / 8 - 1) / (kvq::kThreads / 8), cap = (long long)sm_count() * 8;
-  return (int)(need < cap ? need : cap);
+// Units of 32 rows of one KV head, one block each.
+long long row_units(const core_kvq_t* c, int n_rows) {
+  return (long long)c->batch * c->n_kv_heads * ((n_rows + kvq::kRows - 1) / kvq::kRows);
 }
 
 template <template <typename, int, int> class F, typename T, typename... A>
@@ -479,7 +533,9 @@ extern "C" int core_kvq_quantize(const core_kvq_t* cache, int32_t dtype, const v
   p.counts = counts;
   p.start0 = start_all;
   p.status = device_status();
-  const int blocks = row_blocks((long long)cache->batch * cache->n_kv_heads * n_rows);
+  const long long units = row_units(cache, n_rows);
+  if (units > INT_MAX) return set_error(CORE_ERR_UNSUPPORTED, f + ": too many rows");
+  const int blocks = (int)units;
   if (!by_type<Write>(dtype, cache->bits, cache->group, blocks, static_cast<cudaStream_t>(stream), p))
     return set_error(CORE_ERR_UNSUPPORTED, f + ": dtype must be bf16, f16 or f32");
   const cudaError_t e = cudaGetLastError();
@@ -507,7 +563,9 @@ extern "C" int core_kvq_dequantize(const core_kvq_t* cache, int32_t dtype, int32
   p.start = start;
   p.start0 = start_all;
   p.status = device_status();
-  const int blocks = row_blocks((long long)cache->batch * cache->n_kv_heads * n_rows);
+  const long long units = row_units(cache, n_rows);
+  if (units > INT_MAX) return set_error(CORE_ERR_UNSUPPORTED, f + ": too many rows");
+  const int blocks = (int)units;
   if (!by_type<Read>(dtype, cache->bits, cache->group, blocks, static_cast<cudaStream_t>(stream), p))
     return set_error(CORE_ERR_UNSUPPORTED, f + ": dtype must be bf16, f16 or f32");
   const cudaError_t e = cudaGetLastError();
