@@ -3,25 +3,29 @@
 // memory.
 //
 // A CTA takes 256 rows of one KV head (rows pack the query heads that share it:
-// row = query * G + head), as two tiles of 128, and walks its keys in tiles of
-// 128:
+// row = query * G + head), as two tiles of 128, and walks its keys in tiles of 128:
 //
-//   S_x = Q_x K_j^T      128 x 128 x 128 into TMEM
-//   P_x = exp2(S_x s log2e - m)   f16, written over S_x in TMEM
+//   S   = Q_x K_j^T      128 x 128 x 128 into TMEM, one buffer for both row tiles
+//   P_x = exp2(S s log2e - m)     f16, into TMEM
 //   O_x += P_x V_j       A = P_x from TMEM, B = the V tile (MN-major)
 //
-// Roles: warps 0-3 and 4-7 run the softmax of tile 0 and 1, one thread a row;
-// warps 8-11 read codes from global memory, a tile ahead in registers, and write
-// n s + z as swizzled f16 tiles (two K and two V buffers); one thread of warp 12
-// issues the MMAs.  The two tiles alternate: while one's softmax runs, the tensor
-// cores take the other's P V and next Q K.  Turning codes into f16 costs the same
-// for 256 rows as for one, about a quarter of the instructions that the softmax
-// of the 256 rows takes.
+// TMEM holds O_0, O_1 (256 columns), S (128), P_0 and P_1 (64 each).  A softmax
+// thread takes its row of S into registers at once and gives the buffer up, so
+// the other row tile's scores are computed while it works, and its own next ones
+// are there when it is done: softmax and tensor cores run side by side.  (S and P
+// of a row tile in one buffer made softmax, P V and Q K^T follow one another,
+// 4650 cycles a tile pair; 64-key tiles with two buffers each ran into M 128 x
+// N 64 products taking as long as N 128 ones.)
 //
-// S_x of tile j + 1 is issued behind P_x V_j, so a full S_x also says that O_x
-// holds all earlier tiles: the rare rescale (a maximum that passed by 2^8)
-// needs no wait of its own.  Keys and values are rounded to f16 (2^-11), queries
-// stay exact behind a power of two per row.
+// Roles: warps 0-3 and 4-7 run the softmax of tile 0 and 1, one thread a row;
+// warps 8-11 read codes from global memory, 64 tokens ahead in registers, and
+// write n s + z as swizzled f16 tiles (two K and two V buffers); warps 12 and 13
+// issue the MMAs.  Turning codes into f16 costs the same for 256 rows as for one, about
+// a quarter of the instructions that the softmax of the 256 rows takes.
+//
+// Keys and values are rounded to f16 (2^-11), queries stay exact behind a power
+// of two per row.  The maximum of a row is raised, and O_x rescaled, only when a
+// score passes it by 2^8.
 #include <cuda_bf16.h>
 
 #include "attention_quant.cuh"
@@ -31,16 +35,19 @@ namespace core {
 namespace kvq {
 
 constexpr int kManyThreads = 512;
-constexpr uint32_t kTileB = 128 * kD * 2;  // 32 KB: 128 rows of 128 f16
-constexpr uint32_t kAtomB = kTileB / 2;    // 64 channels of the 128 rows
+constexpr uint32_t kTile = 128 * kD * 2;  // 32 KB: 128 rows (queries or tokens) of 128 f16
+constexpr uint32_t kAtom = kTile / 2;     // 64 channels of the rows
+constexpr uint32_t kHalf = 64 * 128;      // 64 rows of an atom
 
 struct ManySmem {
-  static constexpr uint32_t kQ = 0;                  // two tiles
-  static constexpr uint32_t kK = kQ + 2 * kTileB;    // two buffers
-  static constexpr uint32_t kV = kK + 2 * kTileB;
-  static constexpr uint32_t kBar = kV + 2 * kTileB;
-  static constexpr uint32_t kTotal = kBar + 256;
+  static constexpr uint32_t kQ = 0;               // two tiles
+  static constexpr uint32_t kK = kQ + 2 * kTile;  // two buffers
+  static constexpr uint32_t kV = kK + 2 * kTile;
+  static constexpr uint32_t kBar = kV + 2 * kTile;
+  static constexpr uint32_t kTotal = kBar + 512;
 };
+// TMEM columns
+constexpr uint32_t kColO = 0, kColS = 256, kColP = 384;
 
 template <int kRegs>
 __device__ __forceinline__ void reg_inc() {
@@ -49,6 +56,16 @@ __device__ __forceinline__ void reg_inc() {
 template <int kRegs>
 __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
 
 // D[tmem] (+)= A[tmem] * B[smem desc], kind::f16.
@@ -73,7 +90,71 @@ __device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&r)[3
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// 32 lanes x 16 columns (store and wait).
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n\t"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 lanes x 128 columns.  The second statement holds the wait for both loads and
+// passes the first one's registers through, so that nothing uses them before it.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
+  uint32_t a[64], b[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+      :
+        "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]),
+        "=r"(a[8]), "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]),
+        "=r"(a[16]), "=r"(a[17]), "=r"(a[18]), "=r"(a[19]), "=r"(a[20]), "=r"(a[21]), "=r"(a[22]), "=r"(a[23]),
+        "=r"(a[24]), "=r"(a[25]), "=r"(a[26]), "=r"(a[27]), "=r"(a[28]), "=r"(a[29]), "=r"(a[30]), "=r"(a[31]),
+        "=r"(a[32]), "=r"(a[33]), "=r"(a[34]), "=r"(a[35]), "=r"(a[36]), "=r"(a[37]), "=r"(a[38]), "=r"(a[39]),
+        "=r"(a[40]), "=r"(a[41]), "=r"(a[42]), "=r"(a[43]), "=r"(a[44]), "=r"(a[45]), "=r"(a[46]), "=r"(a[47]),
+        "=r"(a[48]), "=r"(a[49]), "=r"(a[50]), "=r"(a[51]), "=r"(a[52]), "=r"(a[53]), "=r"(a[54]), "=r"(a[55]),
+        "=r"(a[56]), "=r"(a[57]), "=r"(a[58]), "=r"(a[59]), "=r"(a[60]), "=r"(a[61]), "=r"(a[62]), "=r"(a[63])
+      : "r"(taddr)
+      : "memory");
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%128];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      :
+        "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]),
+        "=r"(b[8]), "=r"(b[9]), "=r"(b[10]), "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15]),
+        "=r"(b[16]), "=r"(b[17]), "=r"(b[18]), "=r"(b[19]), "=r"(b[20]), "=r"(b[21]), "=r"(b[22]), "=r"(b[23]),
+        "=r"(b[24]), "=r"(b[25]), "=r"(b[26]), "=r"(b[27]), "=r"(b[28]), "=r"(b[29]), "=r"(b[30]), "=r"(b[31]),
+        "=r"(b[32]), "=r"(b[33]), "=r"(b[34]), "=r"(b[35]), "=r"(b[36]), "=r"(b[37]), "=r"(b[38]), "=r"(b[39]),
+        "=r"(b[40]), "=r"(b[41]), "=r"(b[42]), "=r"(b[43]), "=r"(b[44]), "=r"(b[45]), "=r"(b[46]), "=r"(b[47]),
+        "=r"(b[48]), "=r"(b[49]), "=r"(b[50]), "=r"(b[51]), "=r"(b[52]), "=r"(b[53]), "=r"(b[54]), "=r"(b[55]),
+        "=r"(b[56]), "=r"(b[57]), "=r"(b[58]), "=r"(b[59]), "=r"(b[60]), "=r"(b[61]), "=r"(b[62]), "=r"(b[63]),
+        "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
+        "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]),
+        "+r"(a[16]), "+r"(a[17]), "+r"(a[18]), "+r"(a[19]), "+r"(a[20]), "+r"(a[21]), "+r"(a[22]), "+r"(a[23]),
+        "+r"(a[24]), "+r"(a[25]), "+r"(a[26]), "+r"(a[27]), "+r"(a[28]), "+r"(a[29]), "+r"(a[30]), "+r"(a[31]),
+        "+r"(a[32]), "+r"(a[33]), "+r"(a[34]), "+r"(a[35]), "+r"(a[36]), "+r"(a[37]), "+r"(a[38]), "+r"(a[39]),
+        "+r"(a[40]), "+r"(a[41]), "+r"(a[42]), "+r"(a[43]), "+r"(a[44]), "+r"(a[45]), "+r"(a[46]), "+r"(a[47]),
+        "+r"(a[48]), "+r"(a[49]), "+r"(a[50]), "+r"(a[51]), "+r"(a[52]), "+r"(a[53]), "+r"(a[54]), "+r"(a[55]),
+        "+r"(a[56]), "+r"(a[57]), "+r"(a[58]), "+r"(a[59]), "+r"(a[60]), "+r"(a[61]), "+r"(a[62]), "+r"(a[63])
+      : "r"(taddr + 64u)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    v[i] = __uint_as_float(a[i]);
+    v[64 + i] = __uint_as_float(b[i]);
+  }
+}
 
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -89,17 +170,17 @@ __device__ __forceinline__ void store_chunk(uint32_t dst, const uint32_t* w, __h
   sts128(dst, h[0], h[1], h[2], h[3]);
 }
 
-// One dequantising thread's share of a K tile: rows r0 + 8 i, the 16-byte chunk t
+// One thread's share of 64 tokens of K: rows r0 + 8 i, the 16-byte chunk t
 // (8 bits: t and 4 + t) of each.  Lanes that store together hold rows r and r + 4.
 template <int kBits, int kG>
 struct KeyPiece {
-  uint4 c[4][kBits / 4];
-  uint32_t m[4][kG];
+  uint4 c[2][kBits / 4];
+  uint32_t m[2][kG];
   __device__ __forceinline__ void load(const AttnParams& p, long long row) {
     const int lane = threadIdx.x & 31, t = lane & 3, w = (threadIdx.x >> 5) & 3;
-    const int r0 = w * 32 + (lane >> 3) + (lane & 4);
+    const int r0 = w * 16 + (lane >> 3) + (lane & 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const int r = r0 + 8 * i;
       const uint8_t* src = p.kc + (row + r) * (16 * kBits);
 #pragma unroll
@@ -119,9 +200,9 @@ struct KeyPiece {
   }
   __device__ __forceinline__ void store(uint32_t tile) const {
     const int lane = threadIdx.x & 31, t = lane & 3, w = (threadIdx.x >> 5) & 3;
-    const int r0 = w * 32 + (lane >> 3) + (lane & 4);
+    const int r0 = w * 16 + (lane >> 3) + (lane & 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const int r = r0 + 8 * i;
       const uint32_t rowa = tile + (uint32_t)r * 128u;
 #pragma unroll
@@ -135,7 +216,7 @@ struct KeyPiece {
           x[1] = b & 1 ? u.w : u.y;
         }
         const uint32_t mw = m[i][b * kG / 4];
-        store_chunk<kBits>(rowa + (uint32_t)(b >> 1) * kAtomB + ((uint32_t)(((b & 1) * 4 + t) ^ (r & 7)) << 4), x,
+        store_chunk<kBits>(rowa + (uint32_t)(b >> 1) * kAtom + ((uint32_t)(((b & 1) * 4 + t) ^ (r & 7)) << 4), x,
                            as_half2(prmt(mw, mw, 0x1010)), as_half2(prmt(mw, mw, 0x3232)));
       }
     }
@@ -145,13 +226,13 @@ struct KeyPiece {
 // The same for V: 16 channels of rows r0 + 4 i; a hidden token's row becomes 0.
 template <int kBits, int kG>
 struct ValuePiece {
-  uint32_t c[8][kBits / 2];
-  uint32_t m[8];
+  uint32_t c[4][kBits / 2];
+  uint32_t m[4];
   __device__ __forceinline__ void load(const AttnParams& p, long long row, const uint8_t* mask, int tok0, int end) {
     const int lane = threadIdx.x & 31, g = (lane & 3) + ((lane >> 1) & 4), w = (threadIdx.x >> 5) & 3;
-    const int r0 = w * 32 + ((lane >> 2) & 1) + ((lane >> 3) & 2);
+    const int r0 = w * 16 + ((lane >> 2) & 1) + ((lane >> 3) & 2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int r = r0 + 4 * i;
       const uint8_t* src = p.vc + (row + r) * (16 * kBits);
       if constexpr (kBits == 4) {
@@ -167,11 +248,11 @@ struct ValuePiece {
   }
   __device__ __forceinline__ void store(uint32_t tile) const {
     const int lane = threadIdx.x & 31, g = (lane & 3) + ((lane >> 1) & 4), w = (threadIdx.x >> 5) & 3;
-    const int r0 = w * 32 + ((lane >> 2) & 1) + ((lane >> 3) & 2);
+    const int r0 = w * 16 + ((lane >> 2) & 1) + ((lane >> 3) & 2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int r = r0 + 4 * i;
-      const uint32_t rowa = tile + (uint32_t)(g >> 2) * kAtomB + (uint32_t)r * 128u;
+      const uint32_t rowa = tile + (uint32_t)(g >> 2) * kAtom + (uint32_t)r * 128u;
       const __half2 s = as_half2(prmt(m[i], m[i], 0x1010)), z = as_half2(prmt(m[i], m[i], 0x3232));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -192,11 +273,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
   auto bar_k_empty = [&](int s) { return bar + 32 + 8u * s; };
   auto bar_v_full = [&](int s) { return bar + 48 + 8u * s; };
   auto bar_v_empty = [&](int s) { return bar + 64 + 8u * s; };
-  auto bar_s_full = [&](int x) { return bar + 80 + 8u * x; };
-  auto bar_p_full = [&](int x) { return bar + 96 + 8u * x; };
-  auto bar_o_full = [&](int x) { return bar + 112 + 8u * x; };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + ManySmem::kBar + 200);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + ManySmem::kBar + 208);
+  auto bar_s_full = [&](int x) { return bar + 80 + 8u * x; };   // S holds row tile x's scores
+  auto bar_s_taken = [&](int x) { return bar + 96 + 8u * x; };  // they are in registers
+  auto bar_p_full = [&](int x) { return bar + 112 + 8u * x; };
+  auto bar_pv = [&](int x) { return bar + 128 + 8u * x; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + ManySmem::kBar + 400);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + ManySmem::kBar + 408);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the last row tiles of every head first: under a causal limit they see most
@@ -222,102 +304,136 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_q_full(i), 4);
-      mbar_init(bar_k_full(i), 4);
+      mbar_init(bar_k_full(i), 8);  // four warps, two halves
       mbar_init(bar_k_empty(i), 1);
-      mbar_init(bar_v_full(i), 4);
+      mbar_init(bar_v_full(i), 8);
       mbar_init(bar_v_empty(i), 1);
       mbar_init(bar_s_full(i), 1);
+      mbar_init(bar_s_taken(i), 4);
       mbar_init(bar_p_full(i), 4);
-      mbar_init(bar_o_full(i), 1);
+      mbar_init(bar_pv(i), 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 12) {
-    // S0 [0, 128), S1 [128, 256), O0 [256, 384), O1 [384, 512)
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // All 512 columns are this CTA's, so they start at column 0, lane 0: the address
+  // is a constant, and anything else an error.
+  constexpr uint32_t tmem = 0;
+  if (threadIdx.x == 0 && *tmem_slot != 0) {
+    record_error(p.status, CORE_ERR_CUDA, 1430, (int)*tmem_slot);
+    *abort_flag = 1;
+  }
   auto wait = [&](uint32_t bb, uint32_t parity, int where) -> bool {
     return bounded_wait(bb, parity, abort_flag, p.status, where);
   };
 
   if (warp >= 12) {
     reg_dec<40>();
-    if (warp == 12 && lane == 0) {
-      constexpr uint32_t idesc_qk = (1u << 4) | ((uint32_t)(kManyTok >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-      constexpr uint32_t idesc_pv = idesc_qk | (1u << 16);  // B (the V tile) MN-major
-      auto qk = [&](int x, int j) {
-        const uint32_t k = sK + (uint32_t)(j & 1) * kTileB, q = sQ + (uint32_t)x * kTileB;
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = (uint32_t)(ks >> 2) * kAtomB + (uint32_t)(ks & 3) * 32u;
-          mma_bf16(tmem + 128u * x, sdesc_kmajor(q + off), sdesc_kmajor(k + off), idesc_qk, ks > 0 ? 1u : 0u);
-        }
-        mma_commit(bar_s_full(x));
-      };
-      bool ok = n > 0;
-      for (int x = 0; x < n_x && ok; ++x) ok = wait(bar_q_full(x), 0, 1431);
-      if (ok && (ok = wait(bar_k_full(0), 0, 1432))) {
-        tc_fence_after();
-        for (int x = 0; x < n_x; ++x) qk(x, 0);
-        mma_commit(bar_k_empty(0));
-      }
+    // Two warps issue the MMAs, Q K^T and P V each in its own order, so that
+    // neither waits behind the other's barriers.  A whole warp walks the tiles and
+    // one elected lane issues: addresses and descriptors then stay in uniform
+    // registers, where the MMAs take them (82 cycles an MMA before, 65 now).
+    auto all = [&](uint32_t bb, uint32_t parity, int where) -> bool {
+      const bool got = __all_sync(0xffffffffu, wait(bb, parity, where));
+      tc_fence_after();
+      return got;
+    };
+    bool ok = n > 0;
+    if (warp == 12) {
+      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kManyTok >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      const bool leader = elect_one();
       for (int j = 0; j < n && ok; ++j) {
-        const bool more = j + 1 < n;
-        const int s = j & 1;
-        if (more && !(ok = wait(bar_k_full(s ^ 1), (uint32_t)((j + 1) >> 1) & 1u, 1433))) break;
-        if (!(ok = wait(bar_v_full(s), (uint32_t)(j >> 1) & 1u, 1434))) break;
+        if (!(ok = all(bar_k_full(j & 1), (uint32_t)(j >> 1) & 1u, 1431))) break;
+        const uint64_t kd = sdesc_kmajor(sK + (uint32_t)(j & 1) * kTile);
         for (int x = 0; x < n_x; ++x) {
-          if (!(ok = wait(bar_p_full(x), (uint32_t)j & 1u, 1435))) break;
-          tc_fence_after();
-          for (int ks = 0; ks < 8; ++ks)
-            mma_ts(tmem + 256u + 128u * x, tmem + 128u * x + 8u * ks,
-                   sdesc_sw128(sV + (uint32_t)s * kTileB + (uint32_t)ks * 16u * 128u, kAtomB, 1024u), idesc_pv,
-                   (j > 0 || ks > 0) ? 1u : 0u);
-          if (x == n_x - 1) mma_commit(bar_v_empty(s));
-          if (more) {
-            qk(x, j + 1);
-            if (x == n_x - 1) mma_commit(bar_k_empty(s ^ 1));
-          } else {
-            mma_commit(bar_o_full(x));
+          if (j == 0 && !(ok = all(bar_q_full(x), 0, 1432))) break;
+          // S is free when the row tile before this one has taken its scores
+          const int prev = x > 0 ? 0 : n_x - 1, when = x > 0 ? j : j - 1;
+          if (when >= 0 && !(ok = all(bar_s_taken(prev), (uint32_t)when & 1u, 1433))) break;
+          const uint64_t qd = sdesc_kmajor(sQ + (uint32_t)x * kTile);
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+              const uint32_t off = ((uint32_t)(ks >> 2) * kAtom + (uint32_t)(ks & 3) * 32u) / 16;
+              mma_bf16(tmem + kColS, qd + off, kd + off, idesc, ks > 0 ? 1u : 0u);
+            }
+            mma_commit(bar_s_full(x));
+            if (x == n_x - 1) mma_commit(bar_k_empty(j & 1));
           }
+          __syncwarp();
+        }
+      }
+    } else if (warp == 13) {
+      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24) |
+                                 (1u << 16);  // B (the V tile) MN-major
+      const bool leader = elect_one();
+      for (int j = 0; j < n && ok; ++j) {
+        if (!(ok = all(bar_v_full(j & 1), (uint32_t)(j >> 1) & 1u, 1434))) break;
+        const uint64_t vd = sdesc_sw128(sV + (uint32_t)(j & 1) * kTile, kAtom, 1024u);
+        for (int x = 0; x < n_x; ++x) {
+          if (!(ok = all(bar_p_full(x), (uint32_t)j & 1u, 1435))) break;
+          const uint32_t a = tmem + kColP + 64u * x, d = tmem + kColO + 128u * x;
+          if (leader) {
+            mma_ts(d, a, vd, idesc, j > 0 ? 1u : 0u);
+#pragma unroll
+            for (int ks = 1; ks < 8; ++ks) mma_ts(d, a + 8u * ks, vd + ks * 16 * 128 / 16, idesc, 1u);
+            mma_commit(bar_pv(x));
+            if (x == n_x - 1) mma_commit(bar_v_empty(j & 1));
+          }
+          __syncwarp();
         }
       }
     }
   } else if (warp >= 8) {
     // ---------------- codes to f16 tiles ----------------
-    reg_dec<112>();
+    reg_dec<96>();
     KeyPiece<kBits, kG> kp;
     ValuePiece<kBits, kG> vp;
     bool ok = true;
-    if (n > 0) {
-      kp.load(p, base + (long long)tile0 * kManyTok);
-      vp.load(p, base + (long long)tile0 * kManyTok, mask, tile0 * kManyTok, end);
-    }
-    for (int j = 0; j < n; ++j) {
-      const int s = j & 1, next = (tile0 + j + 1) * kManyTok;
-      if (j >= 2) ok = __all_sync(0xffffffffu, wait(bar_k_empty(s), (uint32_t)((j >> 1) - 1) & 1u, 1441));
-      if (!ok) break;
-      kp.store(sK + (uint32_t)s * kTileB);
+    // 64 tokens at a time, K one tile ahead of V: K_0, then the halves of K_{j+1}
+    // and V_j in turn.  A V tile waits for the P V two tiles back, which is done
+    // before this tile's K is needed.
+    const int first = tile0 * kManyTok;
+    auto put_k = [&](int i) -> bool {  // half tile i
+      const int s = (i >> 1) & 1;
+      if (i >= 4 && (i & 1) == 0) ok = __all_sync(0xffffffffu, wait(bar_k_empty(s), (uint32_t)((i >> 2) - 1) & 1u, 1441));
+      if (!ok) return false;
+      kp.store(sK + (uint32_t)s * kTile + (uint32_t)(i & 1) * kHalf);
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_k_full(s));
-      if (j + 1 < n) kp.load(p, base + next);
-      if (j >= 2) ok = __all_sync(0xffffffffu, wait(bar_v_empty(s), (uint32_t)((j >> 1) - 1) & 1u, 1442));
-      if (!ok) break;
-      vp.store(sV + (uint32_t)s * kTileB);
+      if (i + 1 < 2 * n) kp.load(p, base + first + (i + 1) * 64);
+      return true;
+    };
+    auto put_v = [&](int i) -> bool {
+      const int s = (i >> 1) & 1, next = first + (i + 1) * 64;
+      if (i >= 4 && (i & 1) == 0) ok = __all_sync(0xffffffffu, wait(bar_v_empty(s), (uint32_t)((i >> 2) - 1) & 1u, 1442));
+      if (!ok) return false;
+      vp.store(sV + (uint32_t)s * kTile + (uint32_t)(i & 1) * kHalf);
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_v_full(s));
-      if (j + 1 < n) vp.load(p, base + next, mask, next, end);
+      if (i + 1 < 2 * n) vp.load(p, base + next, mask, next, end);
+      return true;
+    };
+    if (n > 0) {
+      kp.load(p, base + first);
+      vp.load(p, base + first, mask, first, end);
+      if (put_k(0) && put_k(1)) {
+        for (int i = 0; i < 2 * n; ++i)
+          if ((i + 2 < 2 * n && !put_k(i + 2)) || !put_v(i)) break;
+      }
     }
   } else {
     // ---------------- softmax and epilogue: one thread a row ----------------
-    reg_inc<176>();
+    reg_inc<184>();
     const int x = warp >> 2;
     if (x < n_x) {
       const int r = (warp & 3) * 32 + lane;  // row of the tile
@@ -354,7 +470,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
             const float2 f = query_pair(w[e], p.f16 != 0);
             h[e] = as_u32(__floats2half2_rn(f.x * sh.f1 * sh.f2, f.y * sh.f1 * sh.f2));
           }
-          sts128(sQ + (uint32_t)x * kTileB + (uint32_t)(c >> 3) * kAtomB + (uint32_t)r * 128u +
+          sts128(sQ + (uint32_t)x * kTile + (uint32_t)(c >> 3) * kAtom + (uint32_t)r * 128u +
                      ((uint32_t)((c & 7) ^ (r & 7)) << 4),
                  h[0], h[1], h[2], h[3]);
         }
@@ -363,7 +479,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
         if (lane == 0) mbar_arrive(bar_q_full(x));
       }
       const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-      const uint32_t tS = lanes + 128u * x, tO = lanes + 256u + 128u * x;
+      const uint32_t tS = lanes + kColS, tP = lanes + kColP + 64u * x, tO = lanes + kColO + 128u * x;
+      const unsigned long long sc2 = f2_pack(sc, sc);
       float m_used = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < n; ++j) {
@@ -380,59 +497,71 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
         ok = __all_sync(0xffffffffu, wait(bar_s_full(x), (uint32_t)j & 1u, 1451));
         if (!ok) break;
         tc_fence_after();
-        float v[4][32];
-        float mx = -INFINITY;
+        float v[128];
+        tmem_ld128(tS, v);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_s_taken(x));
+        if (!full) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld32(tS + 32u * c, v[c]);
-          if (!full) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((bits[c] >> e) & 1u) || tok0 + 32 * c + e >= lim) v[c][e] = -INFINITY;
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) mx = fmax3(mx, v[c][e], v[c][e + 1]);
+          for (int e = 0; e < 128; ++e)
+            if (!((bits[e >> 5] >> (e & 31)) & 1u) || tok0 + e >= lim) v[e] = -INFINITY;
         }
-        const float mt = mx * sc;
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 128; e += 8) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], v[e + 2 * c], v[e + 2 * c + 1]);
+        }
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         const bool raise = mt > m_used + kRaise;
+        // O_x holds every earlier tile, and P_x may be written again, once the last
+        // P V has landed
+        auto last_pv = [&]() -> bool {
+          const bool got = j == 0 || wait(bar_pv(x), (uint32_t)(j - 1) & 1u, 1452);
+          tc_fence_after();
+          return __all_sync(0xffffffffu, got);
+        };
         if (__any_sync(0xffffffffu, raise)) {
           const float f = raise ? ex2_approx(m_used - mt) : 1.0f;
           if (j > 0) {
+            if (!(ok = last_pv())) break;
             l *= f;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              float o[32];
-              tmem_ld32(tO + 32u * c, o);
+            for (int c = 0; c < 8; ++c) {
+              float o[16];
+              tmem_ld16(tO + 16u * c, o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= f;
-              tmem_st32(tO + 32u * c, o);
+              for (int e = 0; e < 16; ++e) o[e] *= f;
+              tmem_st16(tO + 16u * c, o);
             }
           }
           if (raise) m_used = mt;
         }
         const float neg = m_used == -INFINITY ? 0.f : -m_used;
-        const unsigned long long sc2 = f2_pack(sc, sc), neg2 = f2_pack(neg, neg);
+        const unsigned long long neg2 = f2_pack(neg, neg);
         unsigned long long acc = 0ull;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t h[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const int k = 64 * c + 2 * e;
-            const unsigned long long y = f2_fma(f2_pack(v[k >> 5][k & 31], v[k >> 5][(k & 31) + 1]), sc2, neg2);
+            const unsigned long long y = f2_fma(f2_pack(v[64 * c + 2 * e], v[64 * c + 2 * e + 1]), sc2, neg2);
             const float p0 = ex2_approx(f2_lo(y)), p1 = ex2_approx(f2_hi(y));
             acc = f2_add(acc, f2_pack(p0, p1));
             h[e] = as_u32(__floats2half2_rn(p0, p1));
           }
-          tmem_st32u(tS + 32u * c, h);
+          if (c == 0 && !(ok = last_pv())) break;
+          tmem_st32u(tP + 32u * c, h);
         }
+        if (!ok) break;
         l += f2_lo(acc) + f2_hi(acc);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_p_full(x));
       }
-      if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait(bar_o_full(x), 0, 1452));
+      if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait(bar_pv(x), (uint32_t)(n - 1) & 1u, 1453));
       if (ok) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that saw no token: output 0, LSE -inf
