@@ -45,7 +45,7 @@ template <int kBits, int kG>
 struct Stage {
   static constexpr uint32_t kCodes = kTok * 16 * kBits, kMeta = kTok * 4 * kG;
   static constexpr uint32_t kKc = 0, kVc = kCodes, kKm = 2 * kCodes, kVm = kKm + kMeta, kBytes = kVm + kMeta;
-  static constexpr int kCount = kBits == 4 ? (kG == 4 ? 2 : 3) : 2;
+  static constexpr int kCount = 2;  // more stages gain nothing: 16 warps an SM have 150 KB on the way
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -91,20 +91,28 @@ __device__ __forceinline__ float low_half(uint32_t w) { return __low2float(as_ha
 
 // Query rows [8 nt, 8 nt + 8) of a tile as B operands: lane (g, t) holds of row g
 // the channels 32 b + 8 t .. + 7, in pairs i = 0..3: reg 4 b + i.
-template <int kBits, int kG>
-__device__ __forceinline__ void load_queries(const AttnParams& p, int b, int kvh, int row, int t, uint32_t (&qf)[16],
-                                             uint32_t& qsum, float& row_scale) {
+struct QueryRow {
+  uint4 u[4];
+};
+__device__ __forceinline__ QueryRow load_query(const AttnParams& p, int b, int kvh, int row, int t) {
+  QueryRow r;
   const int i = row / p.G;
-  float x[32];
-  float mx = 0.f;
   const bool live = i < p.Lq;
   const uint16_t* src = static_cast<const uint16_t*>(p.q) + b * p.qb +
                         (long long)(kvh * p.G + (live ? row - i * p.G : 0)) * p.qh + (long long)(live ? i : 0) * p.ql;
 #pragma unroll
+  for (int c = 0; c < 4; ++c)
+    r.u[c] = live ? __ldg(reinterpret_cast<const uint4*>(src + 32 * c + 8 * t)) : make_uint4(0, 0, 0, 0);
+  return r;
+}
+template <int kBits, int kG>
+__device__ __forceinline__ void set_query(const AttnParams& p, const QueryRow& row, int t, uint32_t (&qf)[16],
+                                          uint32_t& qsum, float& row_scale) {
+  float x[32];
+  float mx = 0.f;
+#pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (live) u = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * t);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t w[4] = {row.u[c].x, row.u[c].y, row.u[c].z, row.u[c].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = query_pair(w[j], p.f16 != 0);
@@ -164,6 +172,12 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
   const int row0 = rt * 8 * kNT;
   const int rows = p.G * p.Lq;
 
+  // the queries and the length are asked for first: everything else of the start
+  // happens while they come
+  QueryRow qrow[kNT];
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) qrow[n] = load_query(p, b, kvh, row0 + 8 * n + g, t);
+  const int len = sequence_length(p, b);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWarps * St::kCount; ++i) mbar_init(smem_u32(&bars[i]), 1);
     abort_storage = 0;
@@ -171,12 +185,12 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
   }
   __syncthreads();
 
-  const int len = sequence_length(p, b);
   const int last_row = min(row0 + 8 * kNT, rows) - 1;
   const int end = row_limit(p, last_row, len);  // no row of the tile sees a token from here on
   const int first_end = row_limit(p, row0, len);  // every row sees the tokens before this
   const int per = tiles_per_split(end, kTok, p.n_split);
   const int tile0 = split * per, tile1 = min(tile0 + per, (end + kTok - 1) / kTok);
+  if (p.n_split > 1) launch_dependents();
   if (p.n_split > 1 && tile0 >= tile1 && split > 0) return;  // the join does not read this part
 
   const long long base = (long long)bh * p.cap;
@@ -202,7 +216,7 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     float r;
-    load_queries<kBits, kG>(p, b, kvh, row0 + 8 * n + g, t, qf[n], qsum[n], r);
+    set_query<kBits, kG>(p, qrow[n], t, qf[n], qsum[n], r);
     rs[n][0] = __shfl_sync(0xffffffffu, r, 8 * t);      // row 2 t of the eight
     rs[n][1] = __shfl_sync(0xffffffffu, r, 8 * t + 4);  // row 2 t + 1
     lim[n][0] = row_limit(p, row0 + 8 * n + 2 * t, len);
@@ -540,6 +554,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int 
   const int end = row_limit(p, last_row, len);
   const int per = tiles_per_split(end, tok, p.n_split);
   const int n = per == 0 ? 1 : ((end + tok - 1) / tok + per - 1) / per;
+  wait_primary();
   const float* lse = p.part_lse + row * p.n_split;
   float v[kMaxSplit / 32];
   float m = -INFINITY;
@@ -762,9 +777,20 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
                              : kvq::launch_nt<8, 1>(pl.nt, p, blocks, s);
   if (e != cudaSuccess) return cuda_error(e, pl.many ? "attn_many_kernel launch" : "attn_few_kernel launch");
   if (pl.n_split > 1) {
-    kvq::attn_join_kernel<<<(unsigned)join_blocks, 128, 0, s>>>(p, pl.many ? kvq::kManyRows : 8 * pl.nt,
-                                                                         pl.many ? kvq::kManyTok : kvq::kTok);
-    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_error(e, "attn_join_kernel launch");
+    // the join may be set up while the parts are still computed: it waits for them
+    // on the device
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)join_blocks);
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kvq::attn_join_kernel, p, pl.many ? kvq::kManyRows : 8 * pl.nt,
+                           pl.many ? kvq::kManyTok : kvq::kTok);
+    if (e != cudaSuccess) return cuda_error(e, "attn_join_kernel launch");
   }
   return CORE_OK;
 }

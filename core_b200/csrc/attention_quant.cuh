@@ -85,6 +85,11 @@ __device__ __forceinline__ float2 query_pair(uint32_t w, bool f16) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// Programmatic dependent launch: the kernel of the parts lets the join start, and
+// the join waits there until every part is written.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Sets a kernel's shared memory limits at its first launch on a device: `done`
 // has a bit for each device that has them.
 inline cudaError_t prepare_kernel(const void* kern, uint32_t smem, std::atomic<unsigned long long>& done) {

@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
   const int per = tiles_per_split(end, kManyTok, p.n_split);
   const int tile0 = split * per, tile1 = min(tile0 + per, (end + kManyTok - 1) / kManyTok);
   const int n = max(tile1 - tile0, 0);
+  if (p.n_split > 1) launch_dependents();
   if (n == 0 && split > 0) return;  // the join does not read this part
   const long long base = (long long)bh * p.cap;
   const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (long long)b * p.mask_stride;
