@@ -87,6 +87,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// Four values in the output type.
+__device__ __forceinline__ uint2 half4(float4 x, bool f16) {
+  if (f16) return make_uint2(as_u32(__floats2half2_rn(x.x, x.y)), as_u32(__floats2half2_rn(x.z, x.w)));
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
 __device__ __forceinline__ float low_half(uint32_t w) { return __low2float(as_half2(w)); }
 
 // Query rows [8 nt, 8 nt + 8) of a tile as B operands: lane (g, t) holds of row g
@@ -160,6 +167,7 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
   __shared__ __align__(8) uint64_t bars[kWarps * St::kCount];
   __shared__ int abort_storage;
   __shared__ float sm_m[kWarps][8 * kNT], sm_l[kWarps][8 * kNT];
+  __shared__ long long sm_at[8 * kNT];
   volatile int* abort_flag = &abort_storage;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -471,7 +479,7 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
     if (lane == 0 && it + St::kCount < n_mine) issue(it + St::kCount);
   }
 
-  // ---- join the warps: maxima and sums, then each channel's weighted sum
+  // ---- join the warps: maxima and sums, then each row's weighted mean
 #pragma unroll
   for (int n = 0; n < kNT; ++n)
 #pragma unroll
@@ -500,37 +508,53 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
             make_float4(o[j][n][h], o[j][n][h + 2], o[j + 1][n][h], o[j + 1][n][h + 2]);
       }
     }
-  __syncthreads();
-  const int c = threadIdx.x;
-  for (int r = 0; r < 8 * kNT && row0 + r < rows; ++r) {
-    float m = -INFINITY;
+  if (threadIdx.x < 8 * kNT) {  // one thread a row: the warps' weights, and where the row goes
+    const int r = threadIdx.x, row = row0 + r;
+    float m = -INFINITY, lt = 0.f, f[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm_m[w][r]);
     const float mb = m == -INFINITY ? 0.f : m;
-    float lt = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2_approx(sm_m[w][r] - mb);
-      lt += f * sm_l[w][r];
-      acc += f * so[(w * 8 * kNT + r) * kD + c];
+      f[w] = ex2_approx(sm_m[w][r] - mb);
+      lt += f[w] * sm_l[w][r];
     }
     // a row that saw no token: output 0, LSE -inf.  (NaN scores leave lt NaN.)
-    const float val = lt == 0.f ? 0.f : acc / lt;
+    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) sm_m[w][r] = f[w] * inv;
     const float lse2 = lt == 0.f ? -INFINITY : m + log2f(lt);
-    const int i = (row0 + r) / p.G, hq = kvh * p.G + (row0 + r) - i * p.G;
-    if (p.n_split > 1) {
-      const long long at = ((long long)bh * rows + row0 + r) * p.n_split + split;
-      p.part_o[at * kD + c] = val;
-      if (c == 0) p.part_lse[at] = lse2;
-    } else {
-      const int Hq = p.Hkv * p.G;
-      const long long at = (((long long)b * p.Lq + i) * Hq + hq) * kD + c;
-      if (p.f16)
-        static_cast<__half*>(p.out)[at] = __float2half_rn(val);
-      else
-        static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(val);
-      if (c == 0) p.lse[((long long)b * Hq + hq) * p.Lq + i] = lse2 * 0.69314718055994531f;
+    if (row < rows) {
+      if (p.n_split > 1) {
+        const long long at = ((long long)bh * rows + row) * p.n_split + split;
+        sm_at[r] = at;
+        p.part_lse[at] = lse2;
+      } else {
+        const int i = row / p.G, hq = kvh * p.G + row - i * p.G, Hq = p.Hkv * p.G;
+        sm_at[r] = ((long long)b * p.Lq + i) * Hq + hq;
+        p.lse[((long long)b * Hq + hq) * p.Lq + i] = lse2 * 0.69314718055994531f;
+      }
     }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2 * kNT; ++k) {
+    const int r = warp + kWarps * k;
+    if (row0 + r >= rows) break;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = sm_m[w][r];
+      const float4 x = reinterpret_cast<const float4*>(so + (w * 8 * kNT + r) * kD)[lane];
+      acc.x += f * x.x;
+      acc.y += f * x.y;
+      acc.z += f * x.z;
+      acc.w += f * x.w;
+    }
+    if (p.n_split > 1)
+      reinterpret_cast<float4*>(p.part_o + sm_at[r] * kD)[lane] = acc;
+    else
+      reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + sm_at[r] * kD)[lane] = half4(acc, p.f16);
   }
 }
 
@@ -538,6 +562,7 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
 // four warps takes a row: every warp works out the weights, takes every fourth
 // part, four channels a lane, and the four sums meet in shared memory.
 constexpr int kMaxSplit = 128;
+constexpr bool kForceMany = false, kForceFew = false;
 
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int rows_per_tile, int tok) {
   __shared__ float weight[kMaxSplit];
@@ -617,33 +642,56 @@ int resident(int bits, int group, int nt) {
   return group == 32 ? resident_of<8, 4>(nt) : group == 64 ? resident_of<8, 2>(nt) : resident_of<8, 1>(nt);
 }
 
+// Microseconds that the two kernels take on a B200, as measured over lengths of 1
+// to 131072 and 1 to 2048 rows; the plan only compares them.
+//
+// attn_few_kernel: a CTA starts and ends in about 2.5; a warp takes its tiles one
+// after the other, 1.15 each when it has a scheduler to itself and 0.62 per warp
+// that shares it (two row tiles of eight: 1.4 times that; 8 bits: the bytes bind
+// at 0.8).  The join takes 1.7 and 0.02 a part.
+double few_us(int bits, int resident, int nt, long long units, int tiles, int n) {
+  const long long sms = sm_count(), ctas = units * n;
+  const long long waves = (ctas + sms * resident - 1) / (sms * resident);
+  const long long share = (ctas + sms - 1) / sms < resident ? (ctas + sms - 1) / sms : resident;
+  const int rounds = ((tiles + n - 1) / n + kWarps - 1) / kWarps;
+  const double each = (bits == 4 ? 0.62 : 0.8) * share * (nt == 1 ? 1.0 : 1.4), alone = nt == 1 ? 1.15 : 1.6;
+  return waves * (2.5 + rounds * (each > alone ? each : alone)) + (n > 1 ? 1.7 + 0.02 * n : 0.0);
+}
+// attn_many_kernel: one CTA an SM, 6.5 to start and end, 2.6 a tile of 128 keys
+// (one row tile of 128: 1.9); the join also moves every part's rows.
+double many_us(long long units, long long rows, int tiles, int n) {
+  const long long sms = sm_count(), waves = (units * n + sms - 1) / sms;
+  const double part = 1e-6 * 2 * kD * 4 * units * (rows < kManyRows ? rows : kManyRows) / 3.0;
+  return waves * (6.5 + ((tiles + n - 1) / n) * (rows > 128 ? 2.6 : 1.9)) + (n > 1 ? 1.7 + n * (0.02 + part) : 0.0);
+}
+
 struct Plan {
   bool many;
   int nt, n_rt, n_split;
 };
 
-// Query rows a KV head from which the tcgen05 kernel (256-row tiles) takes over.
-constexpr int kManyFrom = 33;
-
-// Parts of a sequence: the count that ends first when `units` x parts CTAs run
-// in waves, a part costing its tokens plus a fixed start and end.
+// Which kernel takes the call, and into how many parts it cuts the sequences.
 Plan plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
-  Plan r;
-  r.many = rows >= kManyFrom;
-  r.nt = rows <= 8 ? 1 : 2;
-  const int per_tile = r.many ? kManyRows : 8 * r.nt, tok = r.many ? kManyTok : kTok, least = r.many ? 1 : kWarps;
-  r.n_rt = (int)((rows + per_tile - 1) / per_tile);
-  const long long units = (long long)B * Hkv * r.n_rt, slots = (long long)sm_count() * (r.many ? 1 : resident(bits, group, r.nt));
-  const int tiles = (max_len + tok - 1) / tok;
-  const double fixed = r.many ? 4 : 12, join = r.many ? 4 : 8, each = r.many ? 0.2 : 0.1;
+  const long long heads = (long long)B * Hkv;
+  Plan r{};
   double best = 0;
-  r.n_split = 1;
-  for (int n = 1; n <= kMaxSplit && n * least <= (tiles > least ? tiles : least); ++n) {
-    const long long waves = (units * n + slots - 1) / slots;
-    const double cost = (double)waves * ((tiles + n - 1) / n + fixed) + (n > 1 ? join + each * n : 0);
-    if (n == 1 || cost < best) {
-      best = cost;
-      r.n_split = n;
+  const int nt = rows <= 8 ? 1 : 2, res = resident(bits, group, nt);
+  const int few_rt = (int)((rows + 8 * nt - 1) / (8 * nt)), few_tiles = (max_len + kTok - 1) / kTok;
+  for (int n = 1; n <= kMaxSplit && (n == 1 || n * kWarps <= few_tiles); ++n) {
+    const double us = few_us(bits, res, nt, heads * few_rt, few_tiles, n);
+    if (n == 1 || us < best) {
+      best = us;
+      r = {false, nt, few_rt, n};
+    }
+  }
+  // Up to 32 rows stay with the kernel that keeps the keys exact.
+  if ((rows <= 32 && !kForceMany) || kForceFew) return r;
+  const int many_rt = (int)((rows + kManyRows - 1) / kManyRows), many_tiles = (max_len + kManyTok - 1) / kManyTok;
+  for (int n = 1; n <= kMaxSplit && (n == 1 || n <= many_tiles); ++n) {
+    const double us = many_us(heads * many_rt, rows, many_tiles, n);
+    if (us < best || (kForceMany && !r.many)) {
+      best = us;
+      r = {true, 2, many_rt, n};
     }
   }
   return r;
