@@ -645,24 +645,24 @@ int resident(int bits, int group, int nt) {
 // Microseconds that the two kernels take on a B200, as measured over lengths of 1
 // to 131072 and 1 to 2048 rows; the plan only compares them.
 //
-// attn_few_kernel: a CTA starts and ends in about 2.5; a warp takes its tiles one
-// after the other, 1.15 each when it has a scheduler to itself and 0.62 per warp
-// that shares it (two row tiles of eight: 1.4 times that; 8 bits: the bytes bind
-// at 0.8).  The join takes 1.7 and 0.02 a part.
+// attn_few_kernel: 3.3 from launch to end without a tile; a warp takes its tiles
+// one after the other, and a tile takes longer the more CTAs share the SM (1.16,
+// 1.45, 1.94, 2.38 for one to four; 8 bits 1.24, 1.68, 2.65: there the bytes
+// bind).  16 rows: 5 and 1.2 times that.  The join takes 1.8 and 0.03 a part.
 double few_us(int bits, int resident, int nt, long long units, int tiles, int n) {
   const long long sms = sm_count(), ctas = units * n;
   const long long waves = (ctas + sms * resident - 1) / (sms * resident);
   const long long share = (ctas + sms - 1) / sms < resident ? (ctas + sms - 1) / sms : resident;
   const int rounds = ((tiles + n - 1) / n + kWarps - 1) / kWarps;
-  const double each = (bits == 4 ? 0.62 : 0.8) * share * (nt == 1 ? 1.0 : 1.4), alone = nt == 1 ? 1.15 : 1.6;
-  return waves * (2.5 + rounds * (each > alone ? each : alone)) + (n > 1 ? 1.7 + 0.02 * n : 0.0);
+  const double tile = (0.7 + (bits == 4 ? 0.42 : 0.62) * share) * (nt == 1 ? 1.0 : 1.2);
+  return waves * ((nt == 1 ? 3.3 : 5.0) + rounds * tile) + (n > 1 ? 1.8 + 0.03 * n : 0.0);
 }
 // attn_many_kernel: one CTA an SM, 6.5 to start and end, 2.6 a tile of 128 keys
 // (one row tile of 128: 1.9); the join also moves every part's rows.
 double many_us(long long units, long long rows, int tiles, int n) {
   const long long sms = sm_count(), waves = (units * n + sms - 1) / sms;
   const double part = 1e-6 * 2 * kD * 4 * units * (rows < kManyRows ? rows : kManyRows) / 3.0;
-  return waves * (6.5 + ((tiles + n - 1) / n) * (rows > 128 ? 2.6 : 1.9)) + (n > 1 ? 1.7 + n * (0.02 + part) : 0.0);
+  return waves * (6.5 + ((tiles + n - 1) / n) * (rows > 128 ? 2.6 : 1.9)) + (n > 1 ? 1.8 + n * (0.03 + part) : 0.0);
 }
 
 struct Plan {

@@ -93,8 +93,42 @@ class QuantizedKV:
 
     @property
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_meta, self.v_codes,
-                                                          self.v_meta))
+        return sum(t.numel() * t.element_size() for t in self.buffers)
+
+    def reserve(self, capacity: int) -> None:
+        """Room for ``capacity`` tokens a sequence: larger buffers with the same rows."""
+        cap = -(-int(capacity) // CAPACITY_STEP) * CAPACITY_STEP
+        if cap <= self.capacity:
+            return
+        used = -(-self.max_length // CAPACITY_STEP) * CAPACITY_STEP
+        new = []
+        for t in self.buffers:
+            n = t.new_empty((*t.shape[:2], cap, *t.shape[3:]))
+            n[:, :, :used] = t[:, :, :used]
+            new.append(n)
+        self._take(new)
+
+    def select(self, rows: torch.Tensor) -> None:
+        """Keep the sequences ``rows`` (an index along the batch, repeats allowed)."""
+        rows = rows.to(self.device, torch.int64)
+        lengths = self.lengths.index_select(0, rows)
+        self._take([t.index_select(0, rows) for t in self.buffers])
+        self._lengths = lengths
+
+    def crop(self, length: int) -> None:
+        """Forget the tokens from ``length`` on."""
+        length = max(0, int(length))
+        self.lengths.clamp_(max=length)
+        self.max_length = min(self.max_length, length)
+
+    def _take(self, buffers) -> None:
+        lengths, n = self._lengths, self.max_length
+        self.__init__(*buffers)
+        self._lengths, self.max_length = lengths, n
+
+    @property
+    def buffers(self):
+        return self.k_codes, self.k_meta, self.v_codes, self.v_meta
 
     def reset(self) -> None:
         """Forget every token (the buffers stay)."""

@@ -90,6 +90,8 @@ def read_cache_layer(cache, layer_idx: int):
     """(keys, values) of one cache layer, dequantized for a quantized cache
     (kvpress utils.py:98-114: the quantized part only)."""
     layer = cache.layers[layer_idx]
+    if hasattr(layer, "read_rows"):  # core_b200.hf_cache
+        return layer.read_rows()
     if _is_quantized(cache):
         return layer._dequantize(layer._quantized_keys), layer._dequantize(layer._quantized_values)
     return layer.keys, layer.values
@@ -100,6 +102,9 @@ def write_cache_layer(cache, layer_idx: int, keys: torch.Tensor, values: torch.T
     cache re-quantizes them and empties its full-precision residual
     (kvpress base_press.py:146-155)."""
     layer = cache.layers[layer_idx]
+    if hasattr(layer, "write_rows"):  # core_b200.hf_cache
+        layer.write_rows(keys, values)
+        return
     if _is_quantized(cache):
         layer._quantized_keys = layer._quantize(keys, axis=layer.axis_key)
         layer._quantized_values = layer._quantize(values, axis=layer.axis_value)

@@ -1,0 +1,145 @@
+"""The quantised transformers cache under a small random Llama: its layers against
+the rows they stand for, the attention hook on codes against the same cache read
+back, padding, beams, growth, and the press hooks' read and write.
+
+Tolerance of the logits: both sides attend to the same cached values; the hook
+rounds P and the values to f16 where the other rounds them to bf16, and each
+layer's bf16 outputs may differ in the last place (2^-8): over two layers the
+logits agree to 2^-5 of their largest."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch.device("cuda", 0)
+
+
+def _model(dev, impl):
+    from core_b200 import attention
+    from transformers import LlamaConfig, LlamaForCausalLM
+    attention.register()
+    torch.manual_seed(0)
+    cfg = LlamaConfig(vocab_size=97, hidden_size=512, intermediate_size=256, num_hidden_layers=2,
+                      num_attention_heads=4, num_key_value_heads=2, head_dim=128,
+                      max_position_embeddings=4096, attn_implementation=impl)
+    return LlamaForCausalLM(cfg).to(dev, torch.bfloat16).eval()
+
+
+def _steps(model, cache, ids, mask=None, pieces=(1,) * 6):
+    """Logits of the tokens behind the prompt, fed in pieces."""
+    out, at = [], ids.shape[1] - sum(pieces)
+    with torch.no_grad():
+        model(ids[:, :at], past_key_values=cache, attention_mask=None if mask is None else mask[:, :at])
+        for n in pieces:
+            r = model(ids[:, at:at + n], past_key_values=cache,
+                      attention_mask=None if mask is None else mask[:, :at + n])
+            out.append(r.logits)
+            at += n
+    return torch.cat(out, 1).float()
+
+
+@pytest.mark.parametrize("bits,group", [(4, 64), (8, 32)])
+@pytest.mark.parametrize("pieces", [(1,) * 6, (5, 1, 40, 1)])
+def test_codes_against_rows_read_back(bits, group, pieces):
+    from core_b200.hf_cache import QuantizedCacheLayer, quantized_cache
+    dev = _dev()
+    ids = torch.randint(0, 97, (2, 300), generator=torch.Generator().manual_seed(1)).to(dev)
+    model = _model(dev, "core_b200")
+    cache = quantized_cache(model.config, bits=bits, group=group)
+    assert isinstance(cache.layers[0], QuantizedCacheLayer) and cache.layers[0].by_codes
+    a = _steps(model, cache, ids, pieces=pieces)
+    assert cache.get_seq_length() == 300
+    ref = _model(dev, "sdpa")
+    back = quantized_cache(ref.config, bits=bits, group=group)
+    assert not back.layers[0].by_codes
+    b = _steps(ref, back, ids, pieces=pieces)
+    assert (a - b).abs().max() <= 2 ** -5 * b.abs().max()
+
+
+def test_left_padding():
+    from core_b200.hf_cache import quantized_cache
+    dev = _dev()
+    ids = torch.randint(0, 97, (3, 130), generator=torch.Generator().manual_seed(2)).to(dev)
+    mask = torch.ones(3, 130, dtype=torch.long, device=dev)
+    mask[1, :50] = 0
+    mask[2, :7] = 0
+    a = _steps(_model(dev, "core_b200"), quantized_cache(_model(dev, "core_b200").config), ids, mask)
+    ref = _model(dev, "sdpa")
+    b = _steps(ref, quantized_cache(ref.config), ids, mask)
+    assert (a - b).abs().max() <= 2 ** -5 * b.abs().max()
+
+
+def test_generate_and_layer_rows():
+    """generate() with beams runs through reorder_cache; a layer's rows stay within
+    half a step of what was written."""
+    from core_b200.hf_cache import quantized_cache
+    dev = _dev()
+    model = _model(dev, "core_b200")
+    ids = torch.randint(0, 97, (2, 40), generator=torch.Generator().manual_seed(3)).to(dev)
+    cache = quantized_cache(model.config, bits=8, group=32)
+    out = model.generate(ids, past_key_values=cache, max_new_tokens=12, num_beams=2, do_sample=False,
+                         pad_token_id=0, eos_token_id=None)
+    assert out.shape == (2, 52)
+    layer = cache.layers[0]
+    assert layer.kv.batch == 4 and layer.get_seq_length() == 51
+    k, v = layer.read_rows()
+    assert k.shape == (4, 2, 51, 128) and k.dtype == torch.bfloat16 and torch.isfinite(k.float()).all()
+    layer.crop(20)
+    assert layer.get_seq_length() == 20
+    assert torch.equal(layer.read_rows()[0], k[:, :, :20])
+    layer.batch_select_indices(torch.tensor([2, 0]))
+    assert torch.equal(layer.read_rows()[1], v[[2, 0], :, :20])
+    layer.batch_repeat_interleave(2)
+    assert torch.equal(layer.read_rows()[1], v[[2, 2, 0, 0], :, :20])
+
+
+def test_growth_keeps_the_rows():
+    from core_b200.kvcache import QuantizedKV
+    dev = _dev()
+    c = QuantizedKV.empty(2, 2, 128, bits=4, group=32, device=dev)
+    k = torch.randn(2, 2, 300, 128, device=dev, dtype=torch.bfloat16)
+    c.append(k[:, :, :100], -k[:, :, :100])
+    before = c.read()
+    c.reserve(1000)
+    assert c.capacity == 1024 and c.max_length == 100 and c.lengths.tolist() == [100, 100]
+    assert all(torch.equal(x, y) for x, y in zip(before, c.read()))
+    c.append(k[:, :, 100:], -k[:, :, 100:])
+    whole = QuantizedKV.empty(2, 2, 300, bits=4, group=32, device=dev)
+    whole.append(k, -k)
+    assert all(torch.equal(x, y) for x, y in zip(whole.read(), c.read()))
+
+
+def test_press_hooks_read_and_write_rows():
+    from core_b200 import press
+    from core_b200.hf_cache import quantized_cache
+    dev = _dev()
+    model = _model(dev, "core_b200")
+    cache = quantized_cache(model.config)
+    ids = torch.randint(0, 97, (1, 200), generator=torch.Generator().manual_seed(4)).to(dev)
+    with torch.no_grad():
+        model(ids, past_key_values=cache)
+    k, v = press.read_cache_layer(cache, 1)
+    assert k.shape == (1, 2, 200, 128)
+    keep = torch.arange(0, 200, 3, device=dev)
+    press.write_cache_layer(cache, 1, k[:, :, keep], v[:, :, keep])
+    assert cache.layers[1].get_seq_length() == len(keep)
+    k2, v2 = press.read_cache_layer(cache, 1)
+    # re-quantising rows that were read back as bf16 moves them by at most that
+    # rounding and the rounding of their own grid: a step is 1/15 of a group's range
+    step = (k[:, :, keep].float().unflatten(-1, (2, 64)).amax(-1) - k[:, :, keep].float().unflatten(-1, (2, 64)).amin(-1)) / 15
+    err = (k2 - k[:, :, keep]).float().abs().unflatten(-1, (2, 64)).amax(-1)
+    assert (err <= 0.51 * step + 2 ** -7 * k.float().abs().max()).all()
+
+
+def test_refuses_other_head_dims():
+    from core_b200.hf_cache import QuantizedCacheLayer
+    dev = _dev()
+    with pytest.raises(ValueError, match="head_dim"):
+        QuantizedCacheLayer().update(torch.zeros(1, 1, 2, 64, device=dev), torch.zeros(1, 1, 2, 64, device=dev))
+    with pytest.raises(ValueError, match="bits"):
+        QuantizedCacheLayer(bits=3)
