@@ -252,12 +252,18 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
 
   const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (long long)b * p.mask_stride;
   bool ok = true;
+  // this lane's token of the tile, seen or not: asked for a tile ahead
+  auto look = [&](int it) -> uint32_t {
+    const int tok = (tile0 + warp + it * kWarps) * kTok + lane;
+    if (it >= n_mine || tok >= end) return 0u;
+    return mask == nullptr ? 1u : (uint32_t)__ldg(mask + tok);
+  };
+  uint32_t mine = look(0);
   for (int it = 0; it < n_mine; ++it) {
     const int s = it % St::kCount;
     const int tok0 = (tile0 + warp + it * kWarps) * kTok;
-    bool seen = tok0 + lane < end;
-    if (mask != nullptr && seen) seen = mask[tok0 + lane] != 0;
-    const uint32_t bits = __ballot_sync(0xffffffffu, seen);
+    const uint32_t bits = __ballot_sync(0xffffffffu, mine != 0);
+    mine = look(it + 1);
     ok = bounded_wait(my_bars + 8u * s, (uint32_t)(it / St::kCount) & 1u, abort_flag, p.status, 1422);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) {  // give up, but leave no copy of this warp's in flight
@@ -562,7 +568,6 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
 // four warps takes a row: every warp works out the weights, takes every fourth
 // part, four channels a lane, and the four sums meet in shared memory.
 constexpr int kMaxSplit = 128;
-constexpr bool kForceMany = false, kForceFew = false;
 
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int rows_per_tile, int tok) {
   __shared__ float weight[kMaxSplit];
@@ -648,21 +653,23 @@ int resident(int bits, int group, int nt) {
 // attn_few_kernel: 3.3 from launch to end without a tile; a warp takes its tiles
 // one after the other, and a tile takes longer the more CTAs share the SM (1.16,
 // 1.45, 1.94, 2.38 for one to four; 8 bits 1.24, 1.68, 2.65: there the bytes
-// bind).  16 rows: 5 and 1.2 times that.  The join takes 1.8 and 0.03 a part.
+// bind).  16 rows: 5, and 1.2 times that in 4 bits.  The join takes 1.8 and 0.03 a part.
 double few_us(int bits, int resident, int nt, long long units, int tiles, int n) {
   const long long sms = sm_count(), ctas = units * n;
   const long long waves = (ctas + sms * resident - 1) / (sms * resident);
   const long long share = (ctas + sms - 1) / sms < resident ? (ctas + sms - 1) / sms : resident;
   const int rounds = ((tiles + n - 1) / n + kWarps - 1) / kWarps;
-  const double tile = (0.7 + (bits == 4 ? 0.42 : 0.62) * share) * (nt == 1 ? 1.0 : 1.2);
+  const double tile = bits == 8 ? 0.7 + 0.62 * share : (0.7 + 0.42 * share) * (nt == 1 ? 1.0 : 1.2);
   return waves * ((nt == 1 ? 3.3 : 5.0) + rounds * tile) + (n > 1 ? 1.8 + 0.03 * n : 0.0);
 }
-// attn_many_kernel: one CTA an SM, 6.5 to start and end, 2.6 a tile of 128 keys
-// (one row tile of 128: 1.9); the join also moves every part's rows.
-double many_us(long long units, long long rows, int tiles, int n) {
+// attn_many_kernel: one CTA an SM, 8.5 to start and end, 2.65 a tile of 128 keys
+// (one row tile of 128: 2.2; 8 bits: a quarter more); the join also moves every
+// part's rows.
+double many_us(int bits, long long units, long long rows, int tiles, int n) {
   const long long sms = sm_count(), waves = (units * n + sms - 1) / sms;
+  const double tile = (rows > 128 ? 2.65 : 2.2) * (bits == 4 ? 1.0 : 1.25);
   const double part = 1e-6 * 2 * kD * 4 * units * (rows < kManyRows ? rows : kManyRows) / 3.0;
-  return waves * (6.5 + ((tiles + n - 1) / n) * (rows > 128 ? 2.6 : 1.9)) + (n > 1 ? 1.8 + n * (0.03 + part) : 0.0);
+  return waves * (8.5 + ((tiles + n - 1) / n) * tile) + (n > 1 ? 1.8 + n * (0.03 + part) : 0.0);
 }
 
 struct Plan {
@@ -671,30 +678,61 @@ struct Plan {
 };
 
 // Which kernel takes the call, and into how many parts it cuts the sequences.
-Plan plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
-  const long long heads = (long long)B * Hkv;
-  Plan r{};
-  double best = 0;
+// Tried are the counts that fill the SMs once, twice, .. , each lowered to the
+// least that gives its parts as many tiles.
+Plan make_plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
+  const long long heads = (long long)B * Hkv, sms = sm_count();
   const int nt = rows <= 8 ? 1 : 2, res = resident(bits, group, nt);
   const int few_rt = (int)((rows + 8 * nt - 1) / (8 * nt)), few_tiles = (max_len + kTok - 1) / kTok;
-  for (int n = 1; n <= kMaxSplit && (n == 1 || n * kWarps <= few_tiles); ++n) {
-    const double us = few_us(bits, res, nt, heads * few_rt, few_tiles, n);
-    if (n == 1 || us < best) {
+  const long long few_units = heads * few_rt;
+  Plan r{false, nt, few_rt, 1};
+  double best = few_us(bits, res, nt, few_units, few_tiles, 1);
+  auto least = [](int tiles, int step, long long n) {  // same tiles a part (in `step`s), fewest parts
+    const long long most = (tiles + step - 1) / step;
+    n = n < kMaxSplit ? n : kMaxSplit;
+    n = n < most ? n : most;
+    if (n < 2) return 1;
+    const int each = ((tiles + (int)n - 1) / (int)n + step - 1) / step * step;
+    return (tiles + each - 1) / each;
+  };
+  for (int k = 1; k <= 3 * res; ++k) {
+    const int n = least(few_tiles, kWarps, sms * k / few_units);
+    const double us = few_us(bits, res, nt, few_units, few_tiles, n);
+    if (us < best) {
       best = us;
-      r = {false, nt, few_rt, n};
+      r.n_split = n;
     }
   }
   // Up to 32 rows stay with the kernel that keeps the keys exact.
-  if ((rows <= 32 && !kForceMany) || kForceFew) return r;
+  if (rows <= 32) return r;
   const int many_rt = (int)((rows + kManyRows - 1) / kManyRows), many_tiles = (max_len + kManyTok - 1) / kManyTok;
-  for (int n = 1; n <= kMaxSplit && (n == 1 || n <= many_tiles); ++n) {
-    const double us = many_us(heads * many_rt, rows, many_tiles, n);
-    if (us < best || (kForceMany && !r.many)) {
+  const long long many_units = heads * many_rt;
+  for (int k = 0; k <= 6; ++k) {
+    const int n = k == 0 ? 1 : least(many_tiles, 1, sms * k / many_units);
+    const double us = many_us(bits, many_units, rows, many_tiles, n);
+    if (us < best) {
       best = us;
       r = {true, 2, many_rt, n};
     }
   }
   return r;
+}
+
+// The plan of the workspace query serves the call that follows it.
+Plan plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
+  struct Last {
+    long long key[7];
+    Plan plan;
+  };
+  static thread_local Last last{{-1, 0, 0, 0, 0, 0, 0}, {}};
+  const long long key[7] = {bits, group, B, Hkv, rows, max_len, sm_count()};
+  bool same = true;
+  for (int i = 0; i < 7; ++i) same = same && key[i] == last.key[i];
+  if (!same) {
+    last.plan = make_plan(bits, group, B, Hkv, rows, max_len);
+    for (int i = 0; i < 7; ++i) last.key[i] = key[i];
+  }
+  return last.plan;
 }
 
 template <int kBits, int kG, int kNT>

@@ -156,6 +156,29 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
   }
 }
 
+// Loads that stay where they are written: the compiler would otherwise sink them
+// to their first use, a tile later, and leave their latency in the open.
+__device__ __forceinline__ uint4 ldg128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg64(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ldg32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ldg8(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -185,16 +208,16 @@ struct KeyPiece {
       const uint8_t* src = p.kc + (row + r) * (16 * kBits);
 #pragma unroll
       for (int h = 0; h < kBits / 4; ++h)
-        c[i][h] = __ldg(reinterpret_cast<const uint4*>(src + ((64u * h + 16u * t) ^ key_swizzle<kBits>(r))));
+        c[i][h] = ldg128(src + ((64u * h + 16u * t) ^ key_swizzle<kBits>(r)));
       const uint32_t* ms = p.km + (row + r) * kG;
       if constexpr (kG == 4) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(ms));
+        const uint4 x = ldg128(ms);
         m[i][0] = x.x; m[i][1] = x.y; m[i][2] = x.z; m[i][3] = x.w;
       } else if constexpr (kG == 2) {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(ms));
+        const uint2 x = ldg64(ms);
         m[i][0] = x.x; m[i][1] = x.y;
       } else {
-        m[i][0] = __ldg(ms);
+        m[i][0] = ldg32(ms);
       }
     }
   }
@@ -227,7 +250,7 @@ struct KeyPiece {
 template <int kBits, int kG>
 struct ValuePiece {
   uint32_t c[4][kBits / 2];
-  uint32_t m[4];
+  uint32_t m[4], seen[4];
   __device__ __forceinline__ void load(const AttnParams& p, long long row, const uint8_t* mask, int tok0, int end) {
     const int lane = threadIdx.x & 31, g = (lane & 3) + ((lane >> 1) & 4), w = (threadIdx.x >> 5) & 3;
     const int r0 = w * 16 + ((lane >> 2) & 1) + ((lane >> 3) & 2);
@@ -236,14 +259,14 @@ struct ValuePiece {
       const int r = r0 + 4 * i;
       const uint8_t* src = p.vc + (row + r) * (16 * kBits);
       if constexpr (kBits == 4) {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + ((8u * g) ^ value_swizzle<4>(r))));
+        const uint2 x = ldg64(src + ((8u * g) ^ value_swizzle<4>(r)));
         c[i][0] = x.x; c[i][1] = x.y;
       } else {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + ((16u * g) ^ value_swizzle<8>(r))));
+        const uint4 x = ldg128(src + ((16u * g) ^ value_swizzle<8>(r)));
         c[i][0] = x.x; c[i][1] = x.y; c[i][2] = x.z; c[i][3] = x.w;
       }
-      m[i] = __ldg(p.vm + (row + r) * kG + ((g * kG) >> 3));
-      if (tok0 + r >= end || (mask != nullptr && mask[tok0 + r] == 0)) m[i] = 0;
+      m[i] = ldg32(p.vm + (row + r) * kG + ((g * kG) >> 3));
+      seen[i] = tok0 + r >= end ? 0u : mask == nullptr ? 1u : ldg8(mask + tok0 + r);
     }
   }
   __device__ __forceinline__ void store(uint32_t tile) const {
@@ -253,7 +276,8 @@ struct ValuePiece {
     for (int i = 0; i < 4; ++i) {
       const int r = r0 + 4 * i;
       const uint32_t rowa = tile + (uint32_t)(g >> 2) * kAtom + (uint32_t)r * 128u;
-      const __half2 s = as_half2(prmt(m[i], m[i], 0x1010)), z = as_half2(prmt(m[i], m[i], 0x3232));
+      const uint32_t mw = seen[i] ? m[i] : 0u;
+      const __half2 s = as_half2(prmt(mw, mw, 0x1010)), z = as_half2(prmt(mw, mw, 0x3232));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         store_chunk<kBits>(rowa + ((uint32_t)((2 * (g & 3) + h) ^ (r & 7)) << 4), &c[i][h * (kBits / 4)], s, z);
@@ -398,9 +422,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
     KeyPiece<kBits, kG> kp;
     ValuePiece<kBits, kG> vp;
     bool ok = true;
-    // 64 tokens at a time, K one tile ahead of V: K_0, then the halves of K_{j+1}
-    // and V_j in turn.  A V tile waits for the P V two tiles back, which is done
-    // before this tile's K is needed.
+    // 64 tokens at a time, K one tile ahead of V: K_0, then the halves of V_j and
+    // K_{j+1} in turn.  A V tile waits for the P V two tiles back, which is done
+    // before the next tile's K is needed.
     const int first = tile0 * kManyTok;
     auto put_k = [&](int i) -> bool {  // half tile i
       const int s = (i >> 1) & 1;
@@ -429,7 +453,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       vp.load(p, base + first, mask, first, end);
       if (put_k(0) && put_k(1)) {
         for (int i = 0; i < 2 * n; ++i)
-          if ((i + 2 < 2 * n && !put_k(i + 2)) || !put_v(i)) break;
+          if (!put_v(i) || ((i + 2 < 2 * n) && !put_k(i + 2))) break;
       }
     }
   } else {
@@ -484,15 +508,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       const unsigned long long sc2 = f2_pack(sc, sc);
       float m_used = -INFINITY, l = 0.f;
       bool ok = true;
+      // a tile's mask is asked for while the tile before it is worked on
+      uint32_t seen[4] = {1u, 1u, 1u, 1u};
+      auto look = [&](int j) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int k = (tile0 + j) * kManyTok + 32 * c + lane;
+          seen[c] = j < n && k < end ? ldg8(mask + k) : 0u;
+        }
+      };
+      if (mask != nullptr) look(0);
       for (int j = 0; j < n; ++j) {
         const int tok0 = (tile0 + j) * kManyTok;
         uint32_t bits[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
         if (mask != nullptr) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int k = tok0 + 32 * c + lane;
-            bits[c] = __ballot_sync(0xffffffffu, k < end && mask[k] != 0);
-          }
+          for (int c = 0; c < 4; ++c) bits[c] = __ballot_sync(0xffffffffu, seen[c] != 0);
+          look(j + 1);
         }
         const bool full = tok0 + kManyTok <= first && (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
         ok = __all_sync(0xffffffffu, wait(bar_s_full(x), (uint32_t)j & 1u, 1451));

@@ -166,6 +166,7 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
 
 _KVQ_DTYPES = _READOUT_DTYPES
 _I64X3 = ctypes.c_int64 * 3
+_KVQ_SCALE = HEAD_DIM ** -0.5
 
 # One token is written, read or attended to in a few microseconds: these wrappers
 # check in as few calls as they can.
@@ -175,11 +176,10 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _on_device(t: torch.Tensor, cache, name: str) -> None:
-    if t.get_device() != cache.index:
-        if not t.is_cuda:
-            raise ValueError("core_b200 operates on CUDA tensors only (no CPU path)")
-        raise ValueError(f"{name} must be on the cache's device")
+def _wrong_device(t: torch.Tensor, name: str):
+    if not t.is_cuda:
+        return ValueError("core_b200 operates on CUDA tensors only (no CPU path)")
+    return ValueError(f"{name} must be on the cache's device")
 
 
 def _aligned_rows(t: torch.Tensor):
@@ -198,14 +198,18 @@ def _per_sequence(value, cache, name: str):
         return None, int(value)
     if value.shape != (cache.batch,) or value.dtype is not torch.int32 or not value.is_contiguous():
         raise ValueError(f"{name} must be an int or a contiguous (B,) int32 tensor")
-    _on_device(value, cache, name)
+    if value.get_device() != cache.index:
+        raise _wrong_device(value, name)
     return value.data_ptr(), 0
 
 
 def _row_index(index, cache, name: str):
     if index.dim() != 2 or index.shape[0] != cache.batch:
         raise ValueError(f"{name} must be (B, n)")
-    _on_device(index, cache, name)
+    if index.get_device() != cache.index:
+        raise _wrong_device(index, name)
+    if index.dtype is torch.int32 and index.is_contiguous():
+        return index
     return index.to(torch.int32).contiguous()
 
 
@@ -220,8 +224,9 @@ def kv_quantize(keys: torch.Tensor, values: torch.Tensor, cache, start, *,
     only the first counts[b] rows.  Slots or source rows out of range are
     skipped and reported by :func:`status`.
     """
-    _on_device(keys, cache, "keys")
-    _on_device(values, cache, "values")
+    at_device = cache.index
+    if keys.get_device() != at_device or values.get_device() != at_device:
+        raise _wrong_device(values if keys.get_device() == at_device else keys, "keys and values")
     code = _KVQ_DTYPES.get(keys.dtype)
     if code is None or values.dtype is not keys.dtype:
         raise TypeError("kv_quantize takes keys and values of one dtype, bf16, f16 or f32")
@@ -287,16 +292,18 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     Returns (out (B, Lq, Hq, 128) in q's dtype, lse (B, Hq, Lq) f32); a row that
     sees no token gives 0 and -inf.
     """
-    _on_device(q, cache, "q")
+    if q.get_device() != cache.index:
+        raise _wrong_device(q, "q")
     dtype = q.dtype
     code = _ATTN_DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"attention_quantized takes bf16 or f16 queries; got {dtype}")
-    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != HEAD_DIM or q.shape[1] % cache.n_kv_heads:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != cache.batch or shape[3] != HEAD_DIM or shape[1] % cache.n_kv_heads:
         raise ValueError(f"q must be ({cache.batch}, Hq, Lq, {HEAD_DIM}) with Hq a multiple of "
                          f"{cache.n_kv_heads}")
     q, strides = _aligned_rows(q)
-    B, Hq, Lq, _ = q.shape
+    B, Hq, Lq, _ = shape
     at, n = _per_sequence(lengths, cache, "lengths")
     if at is not None:
         n = cache.capacity if max_length is None else int(max_length)
@@ -305,7 +312,8 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
         if (key_mask.dim() != 2 or key_mask.shape[0] != B or key_mask.shape[1] < n
                 or key_mask.dtype not in (torch.bool, torch.uint8)):
             raise ValueError("key_mask must be a (B, >= max_length) bool or uint8 tensor")
-        _on_device(key_mask, cache, "key_mask")
+        if key_mask.get_device() != cache.index:
+            raise _wrong_device(key_mask, "key_mask")
         if key_mask.stride(1) != 1 or (B > 1 and key_mask.stride(0) < key_mask.shape[1]):
             key_mask = key_mask.contiguous()
         mask, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if B > 1 else key_mask.shape[1]
@@ -314,18 +322,20 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     else:
         if out.shape != (B, Lq, Hq, HEAD_DIM) or not out.is_contiguous() or out.dtype is not dtype:
             raise ValueError("out must be a contiguous (B, Lq, Hq, 128) tensor of q's dtype")
-        _on_device(out, cache, "out")
+        if out.get_device() != cache.index:
+            raise _wrong_device(out, "out")
     lse = q.new_empty((B, Hq, Lq), dtype=torch.float32)
     if Lq == 0:
         return out, lse
     lib = _lib.load()
     need = lib.core_kvq_attention_workspace_bytes(cache.handle, Hq, Lq, n)
-    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
-    scale = HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
-    check(lib.core_kvq_attention(
-        cache.handle, code, Hq, Lq, q.data_ptr(), strides, at, n, mask, mask_stride,
-        1 if causal else 0, scale, out.data_ptr(), lse.data_ptr(),
-        None if ws is None else ws.data_ptr(), need, _raw_stream(cache.index)))
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    rc = lib.core_kvq_attention(
+        cache.handle, code, Hq, Lq, q.data_ptr(), strides, at, n, mask, mask_stride, causal,
+        _KVQ_SCALE if softmax_scale is None else softmax_scale, out.data_ptr(), lse.data_ptr(),
+        None if ws is None else ws.data_ptr(), need, _raw_stream(cache.index))
+    if rc:
+        check(rc)
     return out, lse
 
 
