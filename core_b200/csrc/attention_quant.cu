@@ -81,6 +81,9 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
@@ -372,6 +375,14 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
     }
     const bool full = bits == 0xffffffffu && tok0 + kTok <= first_end;
     if (!full) {
+      // hidden tokens: value 0 whatever their bytes hold (scale and zero are
+      // cleared in the tile), score -inf
+      if (!((bits >> lane) & 1u)) {
+#pragma unroll
+        for (int c = 0; c < kG; ++c) sts32(st + St::kVm + (uint32_t)(lane * kG + c) * 4u, 0u);
+      }
+      fence_proxy_async_shared();  // before a copy may take the stage again
+      __syncwarp();
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -437,14 +448,8 @@ __global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kerne
     for (int mt = 0; mt < 2; ++mt) {
       const uint32_t ta = 16 * mt + va, tb = 16 * mt + vb;
       const uint32_t ma = st + St::kVm + vgrp * 4;
-      uint32_t xa = lds32(ma + ta * (4 * kG)), xb = lds32(ma + tb * (4 * kG));
-      uint32_t ya = lds32(ma + (ta + 8) * (4 * kG)), yb = lds32(ma + (tb + 8) * (4 * kG));
-      if (bits != 0xffffffffu) {  // hidden tokens: value 0, whatever their bytes hold
-        xa = (bits >> ta) & 1u ? xa : 0u;
-        xb = (bits >> tb) & 1u ? xb : 0u;
-        ya = (bits >> (ta + 8)) & 1u ? ya : 0u;
-        yb = (bits >> (tb + 8)) & 1u ? yb : 0u;
-      }
+      const uint32_t xa = lds32(ma + ta * (4 * kG)), xb = lds32(ma + tb * (4 * kG));
+      const uint32_t ya = lds32(ma + (ta + 8) * (4 * kG)), yb = lds32(ma + (tb + 8) * (4 * kG));
       const __half2 sx = as_half2(prmt(xa, xb, 0x5410)), zx = as_half2(prmt(xa, xb, 0x7632));
       const __half2 sy = as_half2(prmt(ya, yb, 0x5410)), zy = as_half2(prmt(ya, yb, 0x7632));
       const uint32_t vs = st + St::kVc;
