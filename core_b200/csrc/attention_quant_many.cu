@@ -14,18 +14,29 @@
 // the other row tile's scores are computed while it works, and its own next ones
 // are there when it is done: softmax and tensor cores run side by side.  (S and P
 // of a row tile in one buffer made softmax, P V and Q K^T follow one another,
-// 4650 cycles a tile pair; 64-key tiles with two buffers each ran into M 128 x
-// N 64 products taking as long as N 128 ones.)
+// 4650 cycles a pair of tiles against 3500 now; 64-key tiles with two buffers each
+// ran into M 128 x N 64 products taking as long as N 128 ones.)
 //
-// Roles: warps 0-3 and 4-7 run the softmax of tile 0 and 1, one thread a row;
-// warps 8-11 read codes from global memory, 64 tokens ahead in registers, and
-// write n s + z as swizzled f16 tiles (two K and two V buffers); warps 12 and 13
-// issue the MMAs.  Turning codes into f16 costs the same for 256 rows as for one, about
-// a quarter of the instructions that the softmax of the 256 rows takes.
+// Roles: warps 0-3 and 4-7 run the softmax of row tile 0 and 1, one thread a row;
+// warps 8-11 turn codes into the swizzled f16 tiles of K, warps 12-15 those of V
+// (two buffers each; the codes come 64 tokens ahead in registers); warp 16 issues
+// Q K^T, warp 17 P V.  Turning codes into f16 costs the same for 256 rows as for
+// one, about a third of the instructions that the softmax of the 256 rows takes.
+// With four warps for K and V together that work was the longest chain whenever
+// the codes came from HBM, and the time hung on how far ahead the compiler happened
+// to ask for them (475 to 590 us for 2048 queries over 16384 tokens; 492-522 now,
+// in every format).
 //
-// Keys and values are rounded to f16 (2^-11), queries stay exact behind a power
-// of two per row.  The maximum of a row is raised, and O_x rescaled, only when a
-// score passes it by 2^8.
+// What bounds it now: 512 queries (2048 rows a head) over 16384 tokens take 170 us,
+// 800 TFLOP/s, and 2048 queries 492 us, 1.1 PFLOP/s of the measured 1.65.  A pair
+// of tiles takes about 3500 cycles, of which the MMAs need 2048: Q K^T reads 128
+// bytes of shared memory a cycle, all there are, and shares them with the tiles'
+// writing; the rest is the way of S from tensor core to registers and back.
+//
+// Keys and values are rounded to f16 (2^-11; bf16 would lose three more bits),
+// queries stay exact behind a power of two per row, P is f16 at most 2^8, sums and
+// statistics are f32.  The maximum of a row is raised, and O_x rescaled, only when
+// a score passes it by 2^8.
 #include <cuda_bf16.h>
 
 #include "attention_quant.cuh"
@@ -34,7 +45,7 @@
 namespace core {
 namespace kvq {
 
-constexpr int kManyThreads = 512;
+constexpr int kManyThreads = 640;
 constexpr uint32_t kTile = 128 * kD * 2;  // 32 KB: 128 rows (queries or tokens) of 128 f16
 constexpr uint32_t kAtom = kTile / 2;     // 64 channels of the rows
 constexpr uint32_t kHalf = 64 * 128;      // 64 rows of an atom
@@ -341,7 +352,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
@@ -359,8 +370,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
     return bounded_wait(bb, parity, abort_flag, p.status, where);
   };
 
-  if (warp >= 12) {
-    reg_dec<40>();
+  if (warp >= 16) {
+    reg_dec<32>();
     // Two warps issue the MMAs, Q K^T and P V each in its own order, so that
     // neither waits behind the other's barriers.  A whole warp walks the tiles and
     // one elected lane issues: addresses and descriptors then stay in uniform
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       return got;
     };
     bool ok = n > 0;
-    if (warp == 12) {
+    if (warp == 16) {
       constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kManyTok >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       const bool leader = elect_one();
       for (int j = 0; j < n && ok; ++j) {
@@ -395,7 +406,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
           __syncwarp();
         }
       }
-    } else if (warp == 13) {
+    } else if (warp == 17) {
       constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24) |
                                  (1u << 16);  // B (the V tile) MN-major
       const bool leader = elect_one();
@@ -417,48 +428,37 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       }
     }
   } else if (warp >= 8) {
-    // ---------------- codes to f16 tiles ----------------
-    reg_dec<96>();
-    KeyPiece<kBits, kG> kp;
-    ValuePiece<kBits, kG> vp;
+    // ---------------- codes to f16 tiles: K warps 8-11, V warps 12-15 ----------------
+    reg_dec<56>();
     bool ok = true;
-    // 64 tokens at a time, K one tile ahead of V: K_0, then the halves of V_j and
-    // K_{j+1} in turn.  A V tile waits for the P V two tiles back, which is done
-    // before the next tile's K is needed.
-    const int first = tile0 * kManyTok;
-    auto put_k = [&](int i) -> bool {  // half tile i
-      const int s = (i >> 1) & 1;
-      if (i >= 4 && (i & 1) == 0) ok = __all_sync(0xffffffffu, wait(bar_k_empty(s), (uint32_t)((i >> 2) - 1) & 1u, 1441));
+    const int first = tile0 * kManyTok;  // 64 tokens at a time, the next ones in registers
+    auto put = [&](auto& piece, int i, uint32_t tiles, uint32_t empty, uint32_t full, auto&& get) -> bool {
+      const uint32_t s = (uint32_t)(i >> 1) & 1u;
+      if (i >= 4 && (i & 1) == 0) ok = __all_sync(0xffffffffu, wait(empty + 8u * s, (uint32_t)((i >> 2) - 1) & 1u, 1441));
       if (!ok) return false;
-      kp.store(sK + (uint32_t)s * kTile + (uint32_t)(i & 1) * kHalf);
+      piece.store(tiles + s * kTile + (uint32_t)(i & 1) * kHalf);
       fence_proxy_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_k_full(s));
-      if (i + 1 < 2 * n) kp.load(p, base + first + (i + 1) * 64);
+      if (lane == 0) mbar_arrive(full + 8u * s);
+      if (i + 1 < 2 * n) get(i + 1);
       return true;
     };
-    auto put_v = [&](int i) -> bool {
-      const int s = (i >> 1) & 1, next = first + (i + 1) * 64;
-      if (i >= 4 && (i & 1) == 0) ok = __all_sync(0xffffffffu, wait(bar_v_empty(s), (uint32_t)((i >> 2) - 1) & 1u, 1442));
-      if (!ok) return false;
-      vp.store(sV + (uint32_t)s * kTile + (uint32_t)(i & 1) * kHalf);
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_v_full(s));
-      if (i + 1 < 2 * n) vp.load(p, base + next, mask, next, end);
-      return true;
-    };
-    if (n > 0) {
-      kp.load(p, base + first);
-      vp.load(p, base + first, mask, first, end);
-      if (put_k(0) && put_k(1)) {
-        for (int i = 0; i < 2 * n; ++i)
-          if (!put_v(i) || ((i + 2 < 2 * n) && !put_k(i + 2))) break;
-      }
+    if (n > 0 && warp < 12) {
+      KeyPiece<kBits, kG> piece;
+      auto get = [&](int i) { piece.load(p, base + first + i * 64); };
+      get(0);
+      for (int i = 0; i < 2 * n; ++i)
+        if (!put(piece, i, sK, bar_k_empty(0), bar_k_full(0), get)) break;
+    } else if (n > 0) {
+      ValuePiece<kBits, kG> piece;
+      auto get = [&](int i) { piece.load(p, base + first + i * 64, mask, first + i * 64, end); };
+      get(0);
+      for (int i = 0; i < 2 * n; ++i)
+        if (!put(piece, i, sV, bar_v_empty(0), bar_v_full(0), get)) break;
     }
   } else {
     // ---------------- softmax and epilogue: one thread a row ----------------
-    reg_inc<184>();
+    reg_inc<168>();
     const int x = warp >> 2;
     if (x < n_x) {
       const int r = (warp & 3) * 32 + lane;  // row of the tile
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
