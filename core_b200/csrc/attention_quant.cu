@@ -3,9 +3,13 @@
 //
 //   S = scale q (n s + z)^T,  out = softmax(S) (n s + z),  LSE = log sum exp S
 //
-// What bounds it: the packed cache is read once, 16 bits + 4 (128 / group)
-// bytes a row of K or V; beside that, every code has to be turned into a matrix
-// operand, and at 6.5 TB/s an SM has about two instructions a code to do it.
+// What bounds it: the packed cache is read once, 16 bits + 4 (128 / group) bytes a
+// row of K or V; beside that, every code has to be turned into a matrix operand.
+// In 8 bits the bytes bind: 8 x 32768 tokens of 8 heads 96 us, 5.9 TB/s.  In 4 bits
+// the instructions do: 680 a tile of 32 tokens and warp, issued at 61% of the peak
+// by 16 warps an SM, 68-70 us (4.3-4.9 TB/s); one sequence of 131072 tokens
+// takes 43 us, 24 of them at the rate of memory.  Half of the instructions go
+// through the half-rate integer pipe that masks and pairs the nibbles.
 //
 //  * The codes are the A operand (16 tokens, or 16 channels, a tile) and the
 //    query rows the 8 columns of B, so that a GQA group of up to 8 rows wastes
@@ -23,8 +27,11 @@
 //    bulk copies, running maxima and sums: nothing waits for another warp until
 //    the CTA's four results are joined.  The maximum is raised only when a score
 //    passes it by 2^8.
-//  * A sequence is cut over CTAs when there are few (batch row, KV head) pairs;
-//    a second kernel joins the parts.
+//  * A sequence is cut over CTAs when there are few (batch row, KV head) pairs; a
+//    second kernel, set up while the parts run, joins them.  Which kernel takes a
+//    call and into how many parts is decided by modelled times (below).
+//  * Sums, maxima and the LSE are f32.  P is rounded to f16 (at most 2^8, below
+//    2^-24 of the row's largest it vanishes) and so are V's values; scores are not.
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -638,6 +645,54 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int 
     p.lse[((long long)b * Hq + hq) * p.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
+// The same with a warp a row, for calls with enough rows to fill the SMs that way
+// (a CTA a row spends 400 instructions a warp on each: 33 us for 16384 rows of two
+// parts, 6 us here).
+__global__ void __launch_bounds__(128) attn_join_rows_kernel(const AttnParams p, int rows_per_tile, int tok) {
+  const int rows = p.G * p.Lq;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  wait_primary();
+  if (row >= (long long)p.B * p.Hkv * rows) return;
+  const int bh = (int)(row / rows), r = (int)(row - (long long)bh * rows);
+  const int b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  int len = p.max_len;
+  if (p.lengths != nullptr) len = min(max(p.lengths[b], 0), p.max_len);
+  const int last_row = min(r / rows_per_tile * rows_per_tile + rows_per_tile, rows) - 1;
+  const int end = row_limit(p, last_row, len);
+  const int per = tiles_per_split(end, tok, p.n_split);
+  const int n = per == 0 ? 1 : ((end + tok - 1) / tok + per - 1) / per;
+  const float* lse = p.part_lse + row * p.n_split;
+  const float4* po = reinterpret_cast<const float4*>(p.part_o + row * p.n_split * kD) + lane;
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, lse[i]);
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+  const float mb = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float w = ex2_approx(lse[i] - mb);
+    const float4 x = po[(long long)i * 32];
+    l += w;
+    acc.x += w * x.x;
+    acc.y += w * x.y;
+    acc.z += w * x.z;
+    acc.w += w * x.w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  acc.x *= inv;
+  acc.y *= inv;
+  acc.z *= inv;
+  acc.w *= inv;
+  const int i = r / p.G, hq = kvh * p.G + r - i * p.G, Hq = p.Hkv * p.G;
+  const long long at = ((long long)b * p.Lq + i) * Hq + hq;
+  reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at * kD)[lane] = half4(acc, p.f16);
+  if (lane == 0)
+    p.lse[((long long)b * Hq + hq) * p.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
 // CTAs of attn_few_kernel that fit an SM: by shared memory (228 KB, 1 KB of it
 // the system's for each CTA) and by its launch bounds.
 template <int kBits, int kG>
@@ -851,7 +906,11 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
   carve_parts(c, pl.n_split, rows * p.B * p.Hkv, &p.part_o, &p.part_lse);
   if (c.overflow) return set_error(CORE_ERR_WORKSPACE, f + ": workspace too small");
   const long long blocks = (long long)p.B * p.Hkv * pl.n_rt * pl.n_split;
-  const long long join_blocks = rows * p.B * p.Hkv;
+  // A warp a row where rows are many for their parts, else a CTA a row: 16384 rows of
+  // 2 parts 171 -> 153 us with the attention itself, 2048 rows of 8 parts 31.2 -> 34.9.
+  const long long all_rows = rows * p.B * p.Hkv;
+  const bool join_rows = all_rows > (long long)sm_count() * 8 * pl.n_split;
+  const long long join_blocks = join_rows ? (all_rows + 3) / 4 : all_rows;
   if (blocks > INT_MAX || join_blocks > INT_MAX)
     return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -879,7 +938,7 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kvq::attn_join_kernel, p, pl.many ? kvq::kManyRows : 8 * pl.nt,
+    e = cudaLaunchKernelEx(&cfg, join_rows ? kvq::attn_join_rows_kernel : kvq::attn_join_kernel, p, pl.many ? kvq::kManyRows : 8 * pl.nt,
                            pl.many ? kvq::kManyTok : kvq::kTok);
     if (e != cudaSuccess) return cuda_error(e, "attn_join_kernel launch");
   }

@@ -7,9 +7,17 @@
 //
 // Every step is one correctly rounded f32 operation, so the codes are the same
 // on any machine.  A NaN in a group makes its scale and zero NaN: the group
-// reads back as NaN.  Both kernels move each byte once: eight lanes take a row
-// (16 channels of K and 16 of V each, loaded together), group extrema come from
-// shuffles, and a row's codes leave as 8 or 16 bytes a lane.
+// reads back as NaN.
+//
+// Both kernels move each byte once, eight lanes a row, a block 32 rows of one KV
+// head (no division a row).  Writing: a lane has 16 channels of K and 16 of V in
+// flight, group extrema come from shuffles (16-bit types: least and minus greatest
+// in one register), the codes from shifted sums of the floats' bit patterns, the
+// clamp only for groups that need it.  It is bound by the instructions it issues
+// (460 for 16 channels of K and V a lane, 80% of the issue slots) close to the
+// memory's time: 16384 tokens of 8 heads in bf16 19 us (4.5 TB/s), 8 x 32768 263
+// us (5.4 TB/s).  Reading back is bound by memory: 8 x 32768 tokens 224 us (6.3
+// TB/s), 16384 tokens 16.5 us.
 #include <cuda_bf16.h>
 
 #include <climits>
