@@ -713,14 +713,15 @@ int resident(int bits, int group, int nt) {
 // attn_few_kernel: 3.3 from launch to end without a tile; a warp takes its tiles
 // one after the other, and a tile takes longer the more CTAs share the SM (1.16,
 // 1.45, 1.94, 2.38 for one to four; 8 bits 1.24, 1.68, 2.65: there the bytes
-// bind).  16 rows: 5, and 1.2 times that in 4 bits.  The join takes 1.8 and 0.03 a part.
+// bind).  16 rows: 5, and 1.2 times that in 4 bits.  The join takes 1.8 and 0.03 a
+// part, and its launch 2 more of the caller's time.
 double few_us(int bits, int resident, int nt, long long units, int tiles, int n) {
   const long long sms = sm_count(), ctas = units * n;
   const long long waves = (ctas + sms * resident - 1) / (sms * resident);
   const long long share = (ctas + sms - 1) / sms < resident ? (ctas + sms - 1) / sms : resident;
   const int rounds = ((tiles + n - 1) / n + kWarps - 1) / kWarps;
   const double tile = bits == 8 ? 0.7 + 0.62 * share : (0.7 + 0.42 * share) * (nt == 1 ? 1.0 : 1.2);
-  return waves * ((nt == 1 ? 3.3 : 5.0) + rounds * tile) + (n > 1 ? 1.8 + 0.03 * n : 0.0);
+  return waves * ((nt == 1 ? 3.3 : 5.0) + rounds * tile) + (n > 1 ? 3.8 + 0.03 * n : 0.0);
 }
 // attn_many_kernel: one CTA an SM, 8.5 to start and end, 2.65 a tile of 128 keys
 // (one row tile of 128: 2.2; 8 bits: a quarter more); the join also moves every
@@ -728,8 +729,8 @@ double few_us(int bits, int resident, int nt, long long units, int tiles, int n)
 double many_us(int bits, long long units, long long rows, int tiles, int n) {
   const long long sms = sm_count(), waves = (units * n + sms - 1) / sms;
   const double tile = (rows > 128 ? 2.65 : 2.2) * (bits == 4 ? 1.0 : 1.25);
-  const double part = 1e-6 * 2 * kD * 4 * units * (rows < kManyRows ? rows : kManyRows) / 3.0;
-  return waves * (8.5 + ((tiles + n - 1) / n) * tile) + (n > 1 ? 1.8 + n * (0.03 + part) : 0.0);
+  const double part = 1e-6 * 2 * kD * 4 * units * (rows < kManyRows ? rows : kManyRows) / 5.0;
+  return waves * (8.5 + ((tiles + n - 1) / n) * tile) + (n > 1 ? 3.8 + n * (0.03 + part) : 0.0);
 }
 
 struct Plan {

@@ -332,6 +332,22 @@ def test_attention_lengths(length):
         _check(q, c, lengths, dev)  # bound left at the capacity
 
 
+@pytest.mark.parametrize("lengths", [[5000, 0, 17, 3000, 128, 1], [700] * 5, [0, 0, 0], [1, 2, 4096],
+                                     [(37 * i) % 1500 if i % 7 else 0 for i in range(45)]],
+                         ids=["uneven", "even", "empty", "one_long", "many"])
+def test_attention_ragged_batches(lengths):
+    """Parts dealt out over sequences of unequal lengths, empty ones and more than
+    a warp's worth of them; few and many query rows; a bound far above the lengths."""
+    dev = _dev()
+    B = len(lengths)
+    cap = -(-max(max(lengths), 1) // 128) * 128 + 2048
+    c = _filled(120, B, 1, cap, 4, 64, dev, lengths)
+    for queries in (1, 3, 20):
+        q = _rows(122, (B, 2, queries, 128), torch.float16, 2.0)
+        _check(q, c, lengths, dev, max_length=max(lengths))
+        _check(q, c, lengths, dev)
+
+
 def test_attention_masks():
     """Hidden tokens anywhere, rows that see nothing, NaN and infinities in
     hidden places; bool and uint8 masks, broadcast and strided."""
