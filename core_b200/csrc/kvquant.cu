@@ -9,15 +9,16 @@
 // on any machine.  A NaN in a group makes its scale and zero NaN: the group
 // reads back as NaN.
 //
-// Both kernels move each byte once, eight lanes a row, a block 32 rows of one KV
+// Both kernels move each byte once, eight lanes a row, a block 16 rows of one KV
 // head (no division a row).  Writing: a lane has 16 channels of K and 16 of V in
 // flight, group extrema come from shuffles (16-bit types: least and minus greatest
 // in one register), the codes from shifted sums of the floats' bit patterns, the
 // clamp only for groups that need it.  It is bound by the instructions it issues
 // (460 for 16 channels of K and V a lane, 80% of the issue slots) close to the
-// memory's time: 16384 tokens of 8 heads in bf16 19 us (4.5 TB/s), 8 x 32768 263
-// us (5.4 TB/s).  Reading back is bound by memory: 8 x 32768 tokens 224 us (6.3
-// TB/s), 16384 tokens 16.5 us.
+// memory's time: 16384 tokens of 8 heads in bf16 17.7 us (4.8 TB/s), 8 x 32768 242
+// us (5.8 TB/s).  Reading back is bound by memory: 8 x 32768 tokens 214 us (6.6
+// TB/s), 16384 tokens 16 us.  Blocks of 128 threads, twelve an SM, gave 5% over
+// blocks of 256.
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -160,31 +161,40 @@ __device__ __forceinline__ void pack_codes(const float (&r)[8], uint32_t* w) {
   }
 }
 
-// Codes of eight channels: one word (4 bits) or two (8 bits).
-template <int kBits>
-__device__ __forceinline__ void encode(const float (&x)[8], const Grid& g, uint32_t* w) {
+// Codes of a lane's sixteen channels: two words (4 bits) or four (8 bits).
+template <typename T, int kBits>
+__device__ __forceinline__ void encode(const Piece<T>& p0, const Piece<T>& p1, const Grid& g, uint32_t (&w)[kBits / 2]) {
   constexpr float top = kBits == 4 ? 15.f : 255.f;
   constexpr float magic = 12582912.f;  // 1.5 2^23: adding it rounds to the nearest integer, ties to even
-  float r[8];
+  float x[2][8], r[2][8];
+  p0.get(x[0]);
+  p1.get(x[1]);
   if (g.plain) {
     const unsigned long long nz = f2_pack(-g.z, -g.z), mg = f2_pack(magic, magic);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      // the product is one scalar multiplication a channel: the assembler joins a
-      // packed one with the addition into an fma, whose single rounding moves ties
-      const unsigned long long d = f2_add(f2_pack(x[i], x[i + 1]), nz);
-      const unsigned long long y = f2_add(f2_pack(__fmul_rn(f2_lo(d), g.inv), __fmul_rn(f2_hi(d), g.inv)), mg);
-      r[i] = f2_lo(y);
-      r[i + 1] = f2_hi(y);
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        // the product is one scalar multiplication a channel: the assembler joins a
+        // packed one with the addition into an fma, whose single rounding moves ties
+        const unsigned long long d = f2_add(f2_pack(x[h][i], x[h][i + 1]), nz);
+        const unsigned long long y = f2_add(f2_pack(__fmul_rn(f2_lo(d), g.inv), __fmul_rn(f2_hi(d), g.inv)), mg);
+        r[h][i] = f2_lo(y);
+        r[h][i + 1] = f2_hi(y);
+      }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = fmaxf(fminf(x[i], kLimit), -kLimit);  // NaN: any code, its scale is NaN
-      r[i] = __fadd_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(v, g.z), g.inv), 0.f), top), magic);
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = fmaxf(fminf(x[h][i], kLimit), -kLimit);  // NaN: any code, its scale is NaN
+        r[h][i] = __fadd_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(v, g.z), g.inv), 0.f), top), magic);
+      }
     }
   }
-  pack_codes<kBits>(r, w);
+  pack_codes<kBits>(r[0], w);
+  pack_codes<kBits>(r[1], w + kBits / 4);
 }
 
 // Extrema of 16 channels (or of 8), as a (least, greatest) pair that NaN passes
@@ -261,7 +271,7 @@ struct Extrema<__half> : Extrema16<__half, __half2> {};
 template <>
 struct Extrema<__nv_bfloat16> : Extrema16<__nv_bfloat16, __nv_bfloat162> {};
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kRows = kThreads / 8;  // rows of a block: eight lanes each
 
 // Lane m of a row's eight holds channels 16 m .. 16 m + 15.
@@ -278,11 +288,7 @@ __device__ __forceinline__ void write_row(const Piece<T>& p0, const Piece<T>& p1
   if (kG == 1) e.across(4);
   const Grid g = grid_of<kBits>(e.least(), e.greatest());
   uint32_t w[kBits / 2];
-  float x[8];
-  p0.get(x);
-  encode<kBits>(x, g, w);
-  p1.get(x);
-  encode<kBits>(x, g, w + kBits / 4);
+  encode<T, kBits>(p0, p1, g, w);
   if (!live) return;
   if (keys) {
     // channels 32 b + 8 t .. with b = m / 2 and t = 2 (m & 1), then t + 1
@@ -305,7 +311,7 @@ __device__ __forceinline__ void write_row(const Piece<T>& p0, const Piece<T>& p1
 }
 
 template <typename T, int kBits, int kG>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 8 : 12) quantize_kernel(const WriteParams p) {
   const int m = threadIdx.x & 7;
   const unsigned chunks = ((unsigned)p.T + kRows - 1) / kRows, units = (unsigned)(p.c.B * p.c.H) * chunks;
   // whole warps stay in the loop: the shuffles need every lane of a row
@@ -339,12 +345,27 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const WriteParams p)
   }
 }
 
-// Eight channels n s + z (one rounding in f32) in the output type.
-__device__ __forceinline__ void store8(float* o, const float (&x)[8]) {
-  reinterpret_cast<float4*>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
+// Eight channels in the output type; `apart`: how far the pieces of an even and
+// the next odd lane lie from one another.  f32 pieces of two lanes are exchanged
+// by halves, so that each store covers whole 32-byte sectors (16384 tokens read
+// back as f32: 38 -> 26 us).
+__device__ __forceinline__ void store8(float* o, const float (&x)[8], int apart) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t row = 0xffu << (lane & 24);  // the lanes of a row go the same way
+  const bool odd = lane & 1;
+  float own[4], other[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    own[i] = odd ? x[4 + i] : x[i];
+    other[i] = __shfl_xor_sync(row, odd ? x[i] : x[4 + i], 1);
+  }
+  float* first = odd ? o - apart + 4 : o;   // of the even lane's piece
+  float* second = odd ? o + 4 : o + apart;  // of the odd lane's piece
+  const float4 a = make_float4(own[0], own[1], own[2], own[3]), b = make_float4(other[0], other[1], other[2], other[3]);
+  *reinterpret_cast<float4*>(first) = odd ? b : a;
+  *reinterpret_cast<float4*>(second) = odd ? a : b;
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* o, const float (&x)[8]) {
+__device__ __forceinline__ void store8(__nv_bfloat16* o, const float (&x)[8], int) {
   uint32_t u[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -353,7 +374,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16* o, const float (&x)[8]) {
   }
   *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[2], u[3]);
 }
-__device__ __forceinline__ void store8(__half* o, const float (&x)[8]) {
+__device__ __forceinline__ void store8(__half* o, const float (&x)[8], int) {
   uint32_t u[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) u[i] = as_u32(__floats2half2_rn(x[2 * i], x[2 * i + 1]));
@@ -361,7 +382,7 @@ __device__ __forceinline__ void store8(__half* o, const float (&x)[8]) {
 }
 
 template <typename T, int kBits>
-__device__ __forceinline__ void decode_store(const uint32_t* w, uint32_t meta, T* o) {
+__device__ __forceinline__ void decode_store(const uint32_t* w, uint32_t meta, T* o, int apart) {
   const float2 sz = __half22float2(as_half2(meta));
   float x[8];
 #pragma unroll
@@ -370,11 +391,11 @@ __device__ __forceinline__ void decode_store(const uint32_t* w, uint32_t meta, T
     x[2 * i] = __fmaf_rn(n.x, sz.x, sz.y);
     x[2 * i + 1] = __fmaf_rn(n.y, sz.x, sz.y);
   }
-  store8(o, x);
+  store8(o, x, apart);
 }
 
 template <typename T, int kBits, int kG>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const ReadParams p) {
+__global__ void __launch_bounds__(kThreads, 12) dequantize_kernel(const ReadParams p) {
   const int m = threadIdx.x & 7, a = m >> 2, q = m & 3;
   const unsigned chunks = ((unsigned)p.T + kRows - 1) / kRows, units = (unsigned)(p.c.B * p.c.H) * chunks;
   for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
@@ -393,10 +414,10 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const ReadParams p
     if (slot < 0 || slot >= p.c.cap) {
       if (m == 0) record_error(p.status, CORE_ERR_INVALID_ARG, 1411, t);
       const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      store8(ok, zero);
-      store8(ok + 32, zero);
-      store8(ov, zero);
-      store8(ov + 8, zero);
+      store8(ok, zero, 8);
+      store8(ok + 32, zero, 8);
+      store8(ov, zero, 16);
+      store8(ov + 8, zero, 16);
       continue;
     }
     const long long row = (long long)bh * p.c.cap + slot;
@@ -418,10 +439,10 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const ReadParams p
     }
     const uint32_t k0 = km[kG == 4 ? 2 * a : kG == 2 ? a : 0], k1 = kG == 4 ? km[2 * a + 1] : k0;
     const uint32_t v0 = vm[kG == 4 ? m >> 1 : kG == 2 ? a : 0];
-    decode_store<T, kBits>(kw, k0, ok);
-    decode_store<T, kBits>(kw + kBits / 4, k1, ok + 32);
-    decode_store<T, kBits>(vw, v0, ov);
-    decode_store<T, kBits>(vw + kBits / 4, v0, ov + 8);
+    decode_store<T, kBits>(kw, k0, ok, 8);
+    decode_store<T, kBits>(kw + kBits / 4, k1, ok + 32, 8);
+    decode_store<T, kBits>(vw, v0, ov, 16);
+    decode_store<T, kBits>(vw + kBits / 4, v0, ov + 8, 16);
   }
 }
 
@@ -463,7 +484,7 @@ kvq::Cache device_cache(const core_kvq_t* c) {
   return d;
 }
 
-// Units of 32 rows of one KV head, one block each.
+// Units of kRows rows of one KV head, one block each.
 long long row_units(const core_kvq_t* c, int n_rows) {
   return (long long)c->batch * c->n_kv_heads * ((n_rows + kvq::kRows - 1) / kvq::kRows);
 }

@@ -58,9 +58,10 @@ class QuantizedCacheLayer(CacheLayerMixin):
 
     def _stand_in(self, rows: torch.Tensor) -> torch.Tensor:
         """A tensor of the cached rows' shape without their data, which tells
-        ``attention.attention_forward`` where the codes are."""
+        ``attention.attention_forward`` where the codes are.  It reads as NaN: an
+        attention that does not know it cannot give a plausible result."""
         kv = self.kv
-        t = rows.new_zeros(1).expand(kv.batch, kv.n_kv_heads, kv.max_length, ops.HEAD_DIM)
+        t = rows.new_full((1,), float("nan")).expand(kv.batch, kv.n_kv_heads, kv.max_length, ops.HEAD_DIM)
         setattr(t, attention.CODES, self)
         return t
 

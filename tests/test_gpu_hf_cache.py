@@ -136,6 +136,15 @@ def test_press_hooks_read_and_write_rows():
     assert (err <= 0.51 * step + 2 ** -7 * k.float().abs().max()).all()
 
 
+def test_another_attention_on_codes_is_loud():
+    """A cache made for the hook, handed to an attention that does not know it."""
+    from core_b200.hf_cache import quantized_cache
+    dev = _dev()
+    cache = quantized_cache(_model(dev, "core_b200").config)
+    ids = torch.randint(0, 97, (1, 30), generator=torch.Generator().manual_seed(5)).to(dev)
+    assert _steps(_model(dev, "sdpa"), cache, ids, pieces=(1,)).isnan().all()
+
+
 def test_refuses_other_head_dims():
     from core_b200.hf_cache import QuantizedCacheLayer
     dev = _dev()
