@@ -12,8 +12,8 @@
 // through the half-rate integer pipe that masks and pairs the nibbles.
 //
 //  * The codes are the A operand (16 tokens, or 16 channels, a tile) and the
-//    query rows the 8 columns of B, so that a GQA group of up to 8 rows wastes
-//    little; S^T comes out with a token per row and goes back in as the B
+//    query rows the 8 columns of B (up to three such tiles a CTA), so that a GQA
+//    group of up to 8 rows wastes little; S^T comes out with a token per row and goes back in as the B
 //    operand of P V through movmatrix, without leaving the registers.
 //  * K's codes enter as exact integers: a nibble masked out of its word is the
 //    f16 subnormal n 2^-24 (or 16 n 2^-24; q then carries the 1/16).  A group's
@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnParams p, int 
 }
 
 // The same with a warp a row, for calls with enough rows to fill the SMs that way
-// (a CTA a row spends 400 instructions a warp on each: 33 us for 16384 rows of two
-// parts, 6 us here).
+// (a CTA a row spends 400 instructions a warp on each; with it 512 queries x 32 heads
+// over 16384 tokens, two parts a row, took 171 us instead of 153).
 __global__ void __launch_bounds__(128) attn_join_rows_kernel(const AttnParams p, int rows_per_tile, int tok) {
   const int rows = p.G * p.Lq;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -713,15 +713,17 @@ int resident(int bits, int group, int nt) {
 // attn_few_kernel: 3.3 from launch to end without a tile; a warp takes its tiles
 // one after the other, and a tile takes longer the more CTAs share the SM (1.16,
 // 1.45, 1.94, 2.38 for one to four; 8 bits 1.24, 1.68, 2.65: there the bytes
-// bind).  16 rows: 5, and 1.2 times that in 4 bits.  The join takes 1.8 and 0.03 a
-// part, and its launch 2 more of the caller's time.
+// bind).  16 rows: 5, and 1.2 times that in 4 bits; 24 rows: 7, and 1.75 times (8
+// bits 1.4).  The join takes 1.8 and 0.03 a part, and its launch 2 more of the
+// caller's time.
 double few_us(int bits, int resident, int nt, long long units, int tiles, int n) {
   const long long sms = sm_count(), ctas = units * n;
   const long long waves = (ctas + sms * resident - 1) / (sms * resident);
   const long long share = (ctas + sms - 1) / sms < resident ? (ctas + sms - 1) / sms : resident;
   const int rounds = ((tiles + n - 1) / n + kWarps - 1) / kWarps;
-  const double tile = bits == 8 ? 0.7 + 0.62 * share : (0.7 + 0.42 * share) * (nt == 1 ? 1.0 : 1.2);
-  return waves * ((nt == 1 ? 3.3 : 5.0) + rounds * tile) + (n > 1 ? 3.8 + 0.03 * n : 0.0);
+  const double tile = bits == 8 ? (0.7 + 0.62 * share) * (nt == 3 ? 1.4 : 1.0)
+                                : (0.7 + 0.42 * share) * (nt == 1 ? 1.0 : nt == 2 ? 1.2 : 1.75);
+  return waves * ((nt == 1 ? 3.3 : nt == 2 ? 5.0 : 7.0) + rounds * tile) + (n > 1 ? 3.8 + 0.03 * n : 0.0);
 }
 // attn_many_kernel: one CTA an SM, 8.5 to start and end, 2.65 a tile of 128 keys
 // (one row tile of 128: 2.2; 8 bits: a quarter more); the join also moves every
@@ -743,11 +745,6 @@ struct Plan {
 // least that gives its parts as many tiles.
 Plan make_plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
   const long long heads = (long long)B * Hkv, sms = sm_count();
-  const int nt = rows <= 8 ? 1 : 2, res = resident(bits, group, nt);
-  const int few_rt = (int)((rows + 8 * nt - 1) / (8 * nt)), few_tiles = (max_len + kTok - 1) / kTok;
-  const long long few_units = heads * few_rt;
-  Plan r{false, nt, few_rt, 1};
-  double best = few_us(bits, res, nt, few_units, few_tiles, 1);
   auto least = [](int tiles, int step, long long n) {  // same tiles a part (in `step`s), fewest parts
     const long long most = (tiles + step - 1) / step;
     n = n < kMaxSplit ? n : kMaxSplit;
@@ -756,12 +753,21 @@ Plan make_plan(int bits, int group, int B, int Hkv, long long rows, int max_len)
     const int each = ((tiles + (int)n - 1) / (int)n + step - 1) / step * step;
     return (tiles + each - 1) / each;
   };
-  for (int k = 1; k <= 3 * res; ++k) {
-    const int n = least(few_tiles, kWarps, sms * k / few_units);
-    const double us = few_us(bits, res, nt, few_units, few_tiles, n);
-    if (us < best) {
-      best = us;
-      r.n_split = n;
+  Plan r{};
+  double best = 0;
+  // 8, 16 or 24 rows a CTA: its rows share the codes' turning into operands, but 24
+  // take all 255 registers and a longer start.  24 against 2 x 16 for 20 rows: 44
+  // and 60 us over 8 x 8192 tokens of 8 heads, 12.4 and 11.8 over 1 x 4096.
+  const int few_tiles = (max_len + kTok - 1) / kTok;
+  for (int nt = rows <= 8 ? 1 : 2; nt <= (rows <= 8 ? 1 : rows <= 16 ? 2 : 3); ++nt) {
+    const int res = resident(bits, group, nt), n_rt = (int)((rows + 8 * nt - 1) / (8 * nt));
+    for (int k = 0; k <= 3 * res; ++k) {
+      const int n = k == 0 ? 1 : least(few_tiles, kWarps, sms * k / (heads * n_rt));
+      const double us = few_us(bits, res, nt, heads * n_rt, few_tiles, n);
+      if (r.n_split == 0 || us < best) {
+        best = us;
+        r = {false, nt, n_rt, n};
+      }
     }
   }
   // Up to 32 rows stay with the kernel that keeps the keys exact.
@@ -773,7 +779,7 @@ Plan make_plan(int bits, int group, int B, int Hkv, long long rows, int max_len)
     const double us = many_us(bits, many_units, rows, many_tiles, n);
     if (us < best) {
       best = us;
-      r = {true, 2, many_rt, n};
+      r = {true, 0, many_rt, n};
     }
   }
   return r;
@@ -811,7 +817,9 @@ cudaError_t launch_few(const AttnParams& p, long long blocks, cudaStream_t s) {
 
 template <int kBits, int kG>
 cudaError_t launch_nt(int nt, const AttnParams& p, long long blocks, cudaStream_t s) {
-  return nt == 1 ? launch_few<kBits, kG, 1>(p, blocks, s) : launch_few<kBits, kG, 2>(p, blocks, s);
+  return nt == 1   ? launch_few<kBits, kG, 1>(p, blocks, s)
+         : nt == 2 ? launch_few<kBits, kG, 2>(p, blocks, s)
+                   : launch_few<kBits, kG, 3>(p, blocks, s);
 }
 
 }  // namespace kvq

@@ -332,6 +332,21 @@ def test_attention_lengths(length):
         _check(q, c, lengths, dev)  # bound left at the capacity
 
 
+@pytest.mark.parametrize("bits,group", list(itertools.product((4, 8), (32, 64, 128))))
+@pytest.mark.parametrize("heads,length", [(288, 300), (8, 16001)], ids=["many_heads", "long"])
+def test_attention_three_tiles_of_rows(bits, group, heads, length):
+    """17 to 24 rows a KV head, which one CTA takes together where there are many
+    heads, or long sequences whose parts are joined."""
+    dev = _dev()
+    lengths = [length]
+    c = _filled(140, 1, heads, -(-length // 128) * 128, bits, group, dev, lengths)
+    mask = torch.rand(1, length, generator=torch.Generator().manual_seed(3)) > 0.2
+    for queries in (5, 6):
+        q = _rows(141, (1, 4 * heads, queries, 128), torch.bfloat16, 2.0)
+        _check(q, c, lengths, dev, max_length=length)
+    _check(q, c, lengths, dev, mask=mask, max_length=length)
+
+
 @pytest.mark.parametrize("lengths", [[5000, 0, 17, 3000, 128, 1], [700] * 5, [0, 0, 0], [1, 2, 4096],
                                      [(37 * i) % 1500 if i % 7 else 0 for i in range(45)]],
                          ids=["uneven", "even", "empty", "one_long", "many"])
