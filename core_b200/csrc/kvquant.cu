@@ -536,7 +536,7 @@ extern "C" int core_kvq_quantize(const core_kvq_t* cache, int32_t dtype, const v
   const std::string f(fn);
   if (k == nullptr || v == nullptr || k_strides == nullptr || v_strides == nullptr)
     return set_error(CORE_ERR_INVALID_ARG, f + ": NULL argument");
-  if (src_len <= 0 || n_rows <= 0 || (index == nullptr && n_rows > src_len))
+  if (src_len <= 0 || n_rows <= 0 || n_rows > INT_MAX - 256 || (index == nullptr && n_rows > src_len))
     return set_error(CORE_ERR_INVALID_ARG, f + ": bad row count");
   if (start == nullptr && (start_all < 0 || (int64_t)start_all + n_rows > cache->capacity))
     return set_error(CORE_ERR_INVALID_ARG, f + ": rows outside the cache's capacity");
@@ -578,7 +578,7 @@ extern "C" int core_kvq_dequantize(const core_kvq_t* cache, int32_t dtype, int32
   if (rc != CORE_OK) return rc;
   const std::string f(fn);
   if (out_k == nullptr || out_v == nullptr) return set_error(CORE_ERR_INVALID_ARG, f + ": NULL argument");
-  if (n_rows <= 0) return set_error(CORE_ERR_INVALID_ARG, f + ": bad row count");
+  if (n_rows <= 0 || n_rows > INT_MAX - 256) return set_error(CORE_ERR_INVALID_ARG, f + ": bad row count");
   if (index == nullptr && start == nullptr && (start_all < 0 || (int64_t)start_all + n_rows > cache->capacity))
     return set_error(CORE_ERR_INVALID_ARG, f + ": rows outside the cache's capacity");
   if (!aligned16(out_k) || !aligned16(out_v))

@@ -172,6 +172,10 @@ _KVQ_SCALE = HEAD_DIM ** -0.5
 # check in as few calls as they can.
 
 
+# The C entries launch on the current device: for a cache on another one a wrapper
+# calls itself again with that one current.
+
+
 def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
@@ -208,9 +212,11 @@ def _row_index(index, cache, name: str):
         raise ValueError(f"{name} must be (B, n)")
     if index.get_device() != cache.index:
         raise _wrong_device(index, name)
-    if index.dtype is torch.int32 and index.is_contiguous():
-        return index
-    return index.to(torch.int32).contiguous()
+    if index.dtype is torch.int64:  # what does not fit 32 bits stays out of range
+        index = index.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    elif index.dtype is not torch.int32:
+        raise TypeError(f"{name} must be int32 or int64; got {index.dtype}")
+    return index if index.is_contiguous() else index.contiguous()
 
 
 def kv_quantize(keys: torch.Tensor, values: torch.Tensor, cache, start, *,
@@ -227,6 +233,9 @@ def kv_quantize(keys: torch.Tensor, values: torch.Tensor, cache, start, *,
     at_device = cache.index
     if keys.get_device() != at_device or values.get_device() != at_device:
         raise _wrong_device(values if keys.get_device() == at_device else keys, "keys and values")
+    if torch._C._cuda_getDevice() != at_device:
+        with torch.cuda.device(at_device):
+            return kv_quantize(keys, values, cache, start, index=index, counts=counts)
     code = _KVQ_DTYPES.get(keys.dtype)
     if code is None or values.dtype is not keys.dtype:
         raise TypeError("kv_quantize takes keys and values of one dtype, bf16, f16 or f32")
@@ -258,6 +267,9 @@ def kv_dequantize(cache, *, start=0, count: int | None = None, index: torch.Tens
     """(keys, values) (B, Hkv, n, 128) read back from ``cache``: ``count`` slots
     from ``start`` (an int or a (B,) int32 device tensor), or the slots ``index``
     (B, n).  Each value is n s + z rounded once to ``dtype`` (bf16, f16, f32)."""
+    if torch._C._cuda_getDevice() != cache.index:
+        with torch.cuda.device(cache.index):
+            return kv_dequantize(cache, start=start, count=count, index=index, dtype=dtype)
     code = _KVQ_DTYPES.get(dtype)
     if code is None:
         raise TypeError(f"kv_dequantize gives bf16, f16 or f32; got {dtype}")
@@ -294,6 +306,10 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     """
     if q.get_device() != cache.index:
         raise _wrong_device(q, "q")
+    if torch._C._cuda_getDevice() != cache.index:
+        with torch.cuda.device(cache.index):
+            return attention_quantized(q, cache, lengths, max_length=max_length, key_mask=key_mask,
+                                       softmax_scale=softmax_scale, causal=causal, out=out)
     dtype = q.dtype
     code = _ATTN_DTYPES.get(dtype)
     if code is None:

@@ -577,3 +577,33 @@ def test_refusals():
     e, _ = ops.kv_dequantize(c, count=0)
     assert e.shape == (2, 2, 0, 128)
     ops.status(dev)
+
+
+def test_index_types_and_values_beyond_32_bits():
+    """Indexes are int32 or int64; a value that does not fit 32 bits is out of
+    range, not some other row."""
+    from core_b200 import ops
+    from core_b200._lib import CoreError
+    from core_b200.kvcache import QuantizedKV
+    dev = _dev()
+    c = QuantizedKV.empty(1, 1, 128, device=dev)
+    k = _rows(150, (1, 1, 4, 128), torch.bfloat16).to(dev)
+    c.append(k, k)
+    want = ops.kv_dequantize(c, index=torch.tensor([[2, 0]], dtype=torch.int32, device=dev))[0]
+    assert torch.equal(ops.kv_dequantize(c, index=torch.tensor([[2, 0]], device=dev))[0], want)
+    for far in (2 ** 32 + 1, -2 ** 32 + 1, 2 ** 31):
+        got = ops.kv_dequantize(c, index=torch.tensor([[2, far]], device=dev))[0]
+        assert torch.equal(got[0, 0, 0], want[0, 0, 0]) and (got[0, 0, 1] == 0).all()
+        with pytest.raises(CoreError, match="where=1411"):
+            ops.status(dev)
+        before = c.k_codes.clone()
+        ops.kv_quantize(k, k, c, 4, index=torch.tensor([[far]], device=dev))
+        with pytest.raises(CoreError, match="where=1402"):
+            ops.status(dev)
+        assert torch.equal(c.k_codes, before)
+    for bad in (torch.float32, torch.bool, torch.int16):
+        with pytest.raises(TypeError):
+            ops.kv_dequantize(c, index=torch.zeros(1, 2, device=dev, dtype=bad))
+        with pytest.raises(TypeError):
+            ops.kv_quantize(k, k, c, 0, index=torch.zeros(1, 2, device=dev, dtype=bad))
+    ops.status(dev)

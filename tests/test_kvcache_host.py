@@ -32,3 +32,48 @@ def test_quantised_cache_arguments_rejected_on_host():
     assert "key_mask" in _lib.last_error()
     # one KV head's long sequence is cut into parts: the workspace is missing
     assert attend(cache(cap=4096, heads=1), hq=1, n=4096) == -6
+
+
+def test_row_counts_whose_last_block_passes_31_bits_rejected_on_host():
+    lib = _lib.load()
+    s = ctypes.cast((ctypes.c_int64 * 3)(1 << 20, 1 << 14, 128), ctypes.c_void_p)
+    p, n = ctypes.c_void_p(256), 2 ** 31 - 10
+    cache = ctypes.byref(_lib.CoreKvq(256, 256, 256, 256, 1, 1, 128, 4, 64))
+    assert lib.core_kvq_quantize(cache, _lib.CORE_DTYPE_BF16, p, s, p, s, 4, n, p, p, 0, None, None) == -1
+    assert lib.core_kvq_dequantize(cache, _lib.CORE_DTYPE_BF16, n, p, None, 0, p, p, None) == -1
+
+
+def test_operators_run_with_the_cache_device_current(monkeypatch):
+    """A cache on another device than the current one: the call runs with its
+    device current (torch's switch is a stand-in; each call ends in a refusal
+    that comes after it)."""
+    import contextlib
+    import types
+
+    import pytest
+    import torch
+
+    from core_b200 import ops
+    now, seen = [0], []
+
+    @contextlib.contextmanager
+    def switch(index):
+        before, now[0] = now[0], index
+        seen.append(index)
+        try:
+            yield
+        finally:
+            now[0] = before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", switch)
+    for index in (0, 1):
+        cache = types.SimpleNamespace(index=index)
+        rows = types.SimpleNamespace(get_device=lambda: index, dtype=torch.float64)
+        with pytest.raises(TypeError, match="kv_quantize takes"):
+            ops.kv_quantize(rows, rows, cache, 0)
+        with pytest.raises(TypeError, match="kv_dequantize gives"):
+            ops.kv_dequantize(cache, count=1, dtype=torch.float64)
+        with pytest.raises(TypeError, match="attention_quantized takes"):
+            ops.attention_quantized(rows, cache, 4)
+    assert now == [0] and seen == [1, 1, 1]
