@@ -5,10 +5,10 @@
 //
 // What bounds it: the packed cache is read once, 16 bits + 4 (128 / group) bytes a
 // row of K or V; beside that, every code has to be turned into a matrix operand.
-// In 8 bits the bytes bind: 8 x 32768 tokens of 8 heads 96 us, 5.9 TB/s.  In 4 bits
+// In 8 bits the bytes bind: 8 x 32768 tokens of 8 heads 94 us, 6.0 TB/s.  In 4 bits
 // the instructions do: 680 a tile of 32 tokens and warp, issued at 61% of the peak
-// by 16 warps an SM, 68-70 us (4.3-4.9 TB/s); one sequence of 131072 tokens
-// takes 43 us, 24 of them at the rate of memory.  Half of the instructions go
+// by 16 warps an SM, 67-70 us (4.3-4.9 TB/s); one sequence of 131072 tokens
+// takes 41 us, 24 of them at the rate of memory.  Half of the instructions go
 // through the half-rate integer pipe that masks and pairs the nibbles.
 //
 //  * The codes are the A operand (16 tokens, or 16 channels, a tile) and the
@@ -170,8 +170,8 @@ __device__ __forceinline__ void set_query(const AttnParams& p, const QueryRow& r
   row_scale = p.scale_log2 * 16777216.f * sh.inv1 * sh.inv2;
 }
 
-template <int kBits, int kG, int kNT>
-__global__ void __launch_bounds__(kAttnThreads, kNT == 1 ? 4 : 2) attn_few_kernel(const AttnParams p) {
+template <int kBits, int kG, int kNT, int kCtas>
+__global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const AttnParams p) {
   using St = Stage<kBits, kG>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps * St::kCount];
@@ -693,57 +693,61 @@ __global__ void __launch_bounds__(128) attn_join_rows_kernel(const AttnParams p,
     p.lse[((long long)b * Hq + hq) * p.Lq + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-// CTAs of attn_few_kernel that fit an SM: by shared memory (228 KB, 1 KB of it
-// the system's for each CTA) and by its launch bounds.
-template <int kBits, int kG>
-constexpr int resident_of(int nt) {
-  const int by_smem = 228 * 1024 / (int)(kWarps * Stage<kBits, kG>::kCount * Stage<kBits, kG>::kBytes + 2048);
-  const int by_regs = nt == 1 ? 4 : 2;
-  return by_smem < by_regs ? by_smem : by_regs;
-}
-int resident(int bits, int group, int nt) {
-  if (bits == 4)
-    return group == 32 ? resident_of<4, 4>(nt) : group == 64 ? resident_of<4, 2>(nt) : resident_of<4, 1>(nt);
-  return group == 32 ? resident_of<8, 4>(nt) : group == 64 ? resident_of<8, 2>(nt) : resident_of<8, 1>(nt);
-}
+// CTAs of attn_few_kernel that fit an SM: in 8 bits by shared memory (74 KB each at
+// groups of 32), in 4 bits by registers.
+constexpr int resident(int bits, int nt) { return nt > 1 ? 2 : bits == 8 ? 3 : 4; }
 
 // Microseconds that the two kernels take on a B200, as measured over lengths of 1
 // to 131072 and 1 to 2048 rows; the plan only compares them.
 //
-// attn_few_kernel: 3.3 from launch to end without a tile; a warp takes its tiles
-// one after the other, and a tile takes longer the more CTAs share the SM (1.16,
-// 1.45, 1.94, 2.38 for one to four; 8 bits 1.24, 1.68, 2.65: there the bytes
-// bind).  16 rows: 5, and 1.2 times that in 4 bits; 24 rows: 7, and 1.75 times (8
-// bits 1.4).  The join takes 1.8 and 0.03 a part, and its launch 2 more of the
-// caller's time.
-double few_us(int bits, int resident, int nt, long long units, int tiles, int n) {
-  const long long sms = sm_count(), ctas = units * n;
-  const long long waves = (ctas + sms * resident - 1) / (sms * resident);
-  const long long share = (ctas + sms - 1) / sms < resident ? (ctas + sms - 1) / sms : resident;
-  const int rounds = ((tiles + n - 1) / n + kWarps - 1) / kWarps;
-  const double tile = bits == 8 ? (0.7 + 0.62 * share) * (nt == 3 ? 1.4 : 1.0)
-                                : (0.7 + 0.42 * share) * (nt == 1 ? 1.0 : nt == 2 ? 1.2 : 1.75);
-  return waves * ((nt == 1 ? 3.3 : nt == 2 ? 5.0 : 7.0) + rounds * tile) + (n > 1 ? 3.8 + 0.03 * n : 0.0);
+// attn_few_kernel: the longer of two times, rounded off where they meet (eighth
+// powers).  A warp takes its tiles one after the other, `tile` each; and the SMs
+// together need `all` for each of their tiles, by instructions issued (4 bits) or bytes
+// (8 bits).  Starts grow with the CTAs on an SM, and later waves' are half hidden.
+// Fitted to 600 calls of 333 to 131072 tokens and 2 to 512 sequences x heads; what it
+// picks is 1% off the best of them (24 rows: 4% on top, for they gain little where
+// the other choices are near).
+struct FewTimes {
+  double start, start_cta, tile, all;  // us; all: 1e-3 us over the 148 SMs
+};
+FewTimes few_times(int bits, int nt, int ctas_sm) {
+  if (nt == 3) return bits == 4 ? FewTimes{4.4, 1.8, 1.7, 1.92} : FewTimes{3.9, 2.4, 1.72, 2.14};
+  if (nt == 2) return bits == 4 ? FewTimes{2.7, 1.35, 1.35, 1.33} : FewTimes{2.9, 1.35, 1.3, 1.55};
+  if (bits == 8) return {1.3, 1.0, 1.24, 1.29};
+  return {1.2, 0.9, ctas_sm == 4 ? 1.36 : 1.22, 1.0};
 }
-// attn_many_kernel: one CTA an SM, 8.5 to start and end, 2.65 a tile of 128 keys
-// (one row tile of 128: 2.2; 8 bits: a quarter more); the join also moves every
-// part's rows.
+double few_us(int bits, int ctas_sm, int nt, long long units, int tiles, int n) {
+  const long long sms = sm_count(), ctas = units * n;
+  const long long waves = (ctas + sms * ctas_sm - 1) / (sms * ctas_sm);
+  const long long share = (ctas + sms - 1) / sms < ctas_sm ? (ctas + sms - 1) / sms : ctas_sm;
+  const int rounds = ((tiles + n - 1) / n + kWarps - 1) / kWarps;
+  const FewTimes c = few_times(bits, nt, ctas_sm);
+  auto squared3 = [](double x) { return x *= x, x *= x, x * x; };
+  // SMs wait for fuller ones where instructions bind; memory is one for all
+  const double uneven = bits == 4 ? std::sqrt((double)(waves * share * sms) / ctas) : 1.0;
+  const double in_turn = (double)waves * rounds * c.tile, all = (double)units * tiles * c.all * (0.148 / sms) * uneven;
+  const double body = std::sqrt(std::sqrt(std::sqrt(squared3(in_turn) + squared3(all))));
+  return (0.4 + 0.6 * waves) * (c.start + c.start_cta * share) + body + (n > 1 ? 3.3 + 0.022 * n : 0.0);
+}
+// attn_many_kernel: one CTA an SM; its start and end, and a tile of 128 keys, depend on
+// whether it has one row tile of 128 or two; the join also moves every part's rows.
 double many_us(int bits, long long units, long long rows, int tiles, int n) {
   const long long sms = sm_count(), waves = (units * n + sms - 1) / sms;
-  const double tile = (rows > 128 ? 2.65 : 2.2) * (bits == 4 ? 1.0 : 1.25);
-  const double part = 1e-6 * 2 * kD * 4 * units * (rows < kManyRows ? rows : kManyRows) / 5.0;
-  return waves * (8.5 + ((tiles + n - 1) / n) * tile) + (n > 1 ? 3.8 + n * (0.03 + part) : 0.0);
+  const bool two = rows > 128;
+  const double tile = bits == 8 ? 2.3 : two ? 2.0 : 1.75;
+  const double part = 1e-6 * 2 * kD * 4 * units * (rows < kManyRows ? rows : kManyRows) / 8.0;
+  return waves * ((two ? 14.5 : 9.3) + ((tiles + n - 1) / n) * tile) + (n > 1 ? 3.8 + n * (0.022 + part) : 0.0);
 }
 
 struct Plan {
   bool many;
-  int nt, n_rt, n_split;
+  int nt, ctas, n_rt, n_split;  // few rows: tiles of 8 rows a CTA, CTAs an SM
 };
 
 // Which kernel takes the call, and into how many parts it cuts the sequences.
 // Tried are the counts that fill the SMs once, twice, .. , each lowered to the
 // least that gives its parts as many tiles.
-Plan make_plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
+Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len) {
   const long long heads = (long long)B * Hkv, sms = sm_count();
   auto least = [](int tiles, int step, long long n) {  // same tiles a part (in `step`s), fewest parts
     const long long most = (tiles + step - 1) / step;
@@ -757,16 +761,20 @@ Plan make_plan(int bits, int group, int B, int Hkv, long long rows, int max_len)
   double best = 0;
   // 8, 16 or 24 rows a CTA: its rows share the codes' turning into operands, but 24
   // take all 255 registers and a longer start.  24 against 2 x 16 for 20 rows: 44
-  // and 60 us over 8 x 8192 tokens of 8 heads, 12.4 and 11.8 over 1 x 4096.
+  // and 60 us over 8 x 8192 tokens of 8 heads, 12.4 and 11.8 over 1 x 4096.  8 rows in 4
+  // bits: built for three CTAs an SM or, with 128 registers instead of 168, for four:
+  // 41.3 and 43.4 us over 1 x 131072 tokens, 78.3 and 69.9 over 8 x 32768.
   const int few_tiles = (max_len + kTok - 1) / kTok;
   for (int nt = rows <= 8 ? 1 : 2; nt <= (rows <= 8 ? 1 : rows <= 16 ? 2 : 3); ++nt) {
-    const int res = resident(bits, group, nt), n_rt = (int)((rows + 8 * nt - 1) / (8 * nt));
-    for (int k = 0; k <= 3 * res; ++k) {
-      const int n = k == 0 ? 1 : least(few_tiles, kWarps, sms * k / (heads * n_rt));
-      const double us = few_us(bits, res, nt, heads * n_rt, few_tiles, n);
-      if (r.n_split == 0 || us < best) {
-        best = us;
-        r = {false, nt, n_rt, n};
+    const int most = resident(bits, nt), n_rt = (int)((rows + 8 * nt - 1) / (8 * nt));
+    for (int ctas = most < 3 ? most : 3; ctas <= most; ++ctas) {
+      for (int k = 0; k <= 3 * ctas; ++k) {
+        const int n = k == 0 ? 1 : least(few_tiles, kWarps, sms * k / (heads * n_rt));
+        const double us = few_us(bits, ctas, nt, heads * n_rt, few_tiles, n);
+        if (r.n_split == 0 || us < best) {
+          best = us;
+          r = {false, nt, ctas, n_rt, n};
+        }
       }
     }
   }
@@ -779,35 +787,35 @@ Plan make_plan(int bits, int group, int B, int Hkv, long long rows, int max_len)
     const double us = many_us(bits, many_units, rows, many_tiles, n);
     if (us < best) {
       best = us;
-      r = {true, 0, many_rt, n};
+      r = {true, 0, 1, many_rt, n};
     }
   }
   return r;
 }
 
 // The plan of the workspace query serves the call that follows it.
-Plan plan(int bits, int group, int B, int Hkv, long long rows, int max_len) {
+Plan plan(int bits, int B, int Hkv, long long rows, int max_len) {
   struct Last {
-    long long key[7];
+    long long key[6];
     Plan plan;
   };
-  static thread_local Last last{{-1, 0, 0, 0, 0, 0, 0}, {}};
-  const long long key[7] = {bits, group, B, Hkv, rows, max_len, sm_count()};
+  static thread_local Last last{{-1, 0, 0, 0, 0, 0}, {}};
+  const long long key[6] = {bits, B, Hkv, rows, max_len, sm_count()};
   bool same = true;
-  for (int i = 0; i < 7; ++i) same = same && key[i] == last.key[i];
+  for (int i = 0; i < 6; ++i) same = same && key[i] == last.key[i];
   if (!same) {
-    last.plan = make_plan(bits, group, B, Hkv, rows, max_len);
-    for (int i = 0; i < 7; ++i) last.key[i] = key[i];
+    last.plan = make_plan(bits, B, Hkv, rows, max_len);
+    for (int i = 0; i < 6; ++i) last.key[i] = key[i];
   }
   return last.plan;
 }
 
-template <int kBits, int kG, int kNT>
+template <int kBits, int kG, int kNT, int kCtas = resident(kBits, kNT)>
 cudaError_t launch_few(const AttnParams& p, long long blocks, cudaStream_t s) {
   using St = Stage<kBits, kG>;
   constexpr uint32_t ring = kWarps * St::kCount * St::kBytes, join = kWarps * 8 * kNT * kD * 4;
   constexpr uint32_t smem = ring > join ? ring : join;
-  auto kern = attn_few_kernel<kBits, kG, kNT>;
+  auto kern = attn_few_kernel<kBits, kG, kNT, kCtas>;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = prepare_kernel(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
@@ -816,10 +824,11 @@ cudaError_t launch_few(const AttnParams& p, long long blocks, cudaStream_t s) {
 }
 
 template <int kBits, int kG>
-cudaError_t launch_nt(int nt, const AttnParams& p, long long blocks, cudaStream_t s) {
-  return nt == 1   ? launch_few<kBits, kG, 1>(p, blocks, s)
-         : nt == 2 ? launch_few<kBits, kG, 2>(p, blocks, s)
-                   : launch_few<kBits, kG, 3>(p, blocks, s);
+cudaError_t launch_nt(const Plan& pl, const AttnParams& p, long long blocks, cudaStream_t s) {
+  if (pl.nt == 3) return launch_few<kBits, kG, 3>(p, blocks, s);
+  if (pl.nt == 2) return launch_few<kBits, kG, 2>(p, blocks, s);
+  if (pl.ctas == 3) return launch_few<kBits, kG, 1, 3>(p, blocks, s);
+  return launch_few<kBits, kG, 1>(p, blocks, s);
 }
 
 }  // namespace kvq
@@ -849,7 +858,7 @@ extern "C" size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, in
       cache->batch <= 0 || max_length < 0)
     return 0;
   const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
-  const kvq::Plan pl = kvq::plan(cache->bits, cache->group, cache->batch, cache->n_kv_heads, rows, max_length);
+  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length);
   SizerOut z;
   float *a, *b;
   carve_parts(z, pl.n_split, rows * cache->batch * cache->n_kv_heads, &a, &b);
@@ -908,7 +917,7 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
   p.out = out;
   p.lse = lse;
   p.status = device_status();
-  const kvq::Plan pl = kvq::plan(cache->bits, cache->group, p.B, p.Hkv, rows, max_length);
+  const kvq::Plan pl = kvq::plan(cache->bits, p.B, p.Hkv, rows, max_length);
   p.n_rt = pl.n_rt;
   p.n_split = pl.n_split;
   Carver c(workspace, workspace_bytes);
@@ -927,13 +936,13 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
   if (pl.many)
     e = kvq::launch_many(cache->bits, cache->group, p, blocks, s);
   else if (cache->bits == 4)
-    e = cache->group == 32   ? kvq::launch_nt<4, 4>(pl.nt, p, blocks, s)
-        : cache->group == 64 ? kvq::launch_nt<4, 2>(pl.nt, p, blocks, s)
-                             : kvq::launch_nt<4, 1>(pl.nt, p, blocks, s);
+    e = cache->group == 32   ? kvq::launch_nt<4, 4>(pl, p, blocks, s)
+        : cache->group == 64 ? kvq::launch_nt<4, 2>(pl, p, blocks, s)
+                             : kvq::launch_nt<4, 1>(pl, p, blocks, s);
   else
-    e = cache->group == 32   ? kvq::launch_nt<8, 4>(pl.nt, p, blocks, s)
-        : cache->group == 64 ? kvq::launch_nt<8, 2>(pl.nt, p, blocks, s)
-                             : kvq::launch_nt<8, 1>(pl.nt, p, blocks, s);
+    e = cache->group == 32   ? kvq::launch_nt<8, 4>(pl, p, blocks, s)
+        : cache->group == 64 ? kvq::launch_nt<8, 2>(pl, p, blocks, s)
+                             : kvq::launch_nt<8, 1>(pl, p, blocks, s);
   if (e != cudaSuccess) return cuda_error(e, pl.many ? "attn_many_kernel launch" : "attn_few_kernel launch");
   if (pl.n_split > 1) {
     // the join may be set up while the parts are still computed: it waits for them

@@ -347,6 +347,16 @@ def test_attention_three_tiles_of_rows(bits, group, heads, length):
     _check(q, c, lengths, dev, mask=mask, max_length=length)
 
 
+@pytest.mark.parametrize("bits,group", list(itertools.product((4, 8), (32, 64, 128))))
+def test_attention_full_device(bits, group):
+    """Few rows and enough heads to fill every SM: single tokens of a large batch."""
+    dev = _dev()
+    lengths = [200, 0, 131, 64]
+    c = _filled(160, 4, 140, 256, bits, group, dev, lengths)
+    _check(_rows(162, (4, 280, 1, 128), torch.bfloat16, 2.0), c, lengths, dev, max_length=200)
+    _check(_rows(163, (4, 280, 3, 128), torch.float16, 2.0), c, lengths, dev, max_length=200)
+
+
 @pytest.mark.parametrize("lengths", [[5000, 0, 17, 3000, 128, 1], [700] * 5, [0, 0, 0], [1, 2, 4096],
                                      [(37 * i) % 1500 if i % 7 else 0 for i in range(45)]],
                          ids=["uneven", "even", "empty", "one_long", "many"])
