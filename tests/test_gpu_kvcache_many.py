@@ -1,0 +1,85 @@
+"""Attention over the quantised cache at sizes that the many-row kernel takes, every
+value and LSE against a plain f64 computation.
+
+Tolerances.  K, V and P are rounded to f16 (relative 2^-11 at most, 0.41 of it in the
+mean square).  A score is then off by 2^-11 scale sum|q||k| at most, which moves the
+output by twice that times max|v| beside P's and V's 2^-10 max|v|, and the LSE by as much.
+Each weight and value is off by an independent relative error, so the error's norm stands
+to the output's as one term's to 1: with sqrt(sum q^2 k^2) scale below 2.5 for these
+inputs it is sqrt(2.5^2 + 2) 0.41 2^-11 < 2^-10, and 2^-9 leaves a factor of two; the output's
+rounding adds 2^-9 (bf16) or 2^-12 (f16).  The mean of the LSE's error stays below the
+scores' mean square, 2.5 0.41 2^-11 < 2^-10."""
+
+import itertools
+
+import pytest
+import torch
+
+from test_gpu_kvcache import DT, _decode, _dev, _filled, _rows
+
+pytestmark = pytest.mark.gpu
+
+
+def _reference(q, cache, lengths, mask, causal, scale):
+    """f64 (out (B, Lq, Hq, 128), lse (B, Hq, Lq), largest scale sum|q||k|, largest |v|) on q's device."""
+    K, V = (x.to(q.device) for x in _decode(cache))
+    B, Hq, Lq, _ = q.shape
+    H = cache.n_kv_heads
+    out = torch.zeros(B, Lq, Hq, 128, dtype=torch.float64, device=q.device)
+    lse = torch.full((B, Hq, Lq), -float("inf"), dtype=torch.float64, device=q.device)
+    bound = vmax = 0.0
+    for b in range(B):
+        n = int(lengths[b])
+        see = torch.arange(n, device=q.device).expand(Lq, n)
+        see = see <= torch.arange(n - Lq, n, device=q.device)[:, None] if causal else see >= 0
+        if mask is not None:
+            see = see & mask[b, :n].bool()
+        some = see.any(1)
+        if not some.any():
+            continue
+        # what no query sees may hold anything
+        k, v = (torch.where(see.any(0)[:, None], x[b, :, :n], 0.0) for x in (K, V))
+        k, v = (x.repeat_interleave(Hq // H, 0) for x in (k, v))
+        qq = q[b].double()
+        s = (qq @ k.transpose(1, 2) * scale).masked_fill(~see, -float("inf"))[:, some]
+        lse[b][:, some] = torch.logsumexp(s, 2)
+        out[b, some] = (torch.softmax(s, 2) @ v).transpose(0, 1)
+        bound = max(bound, float((qq.abs() @ k.abs().transpose(1, 2)).max()) * scale)
+        vmax = max(vmax, float(v.abs().max()))
+    return out, lse, bound, vmax
+
+
+def _check_many(q, cache, lengths, *, mask=None, causal=True, scale=128 ** -0.5):
+    from core_b200 import ops
+    at = torch.tensor(lengths, dtype=torch.int32, device=q.device)
+    out, lse = ops.attention_quantized(q, cache, at, max_length=max(lengths), key_mask=mask, causal=causal,
+                                       softmax_scale=scale)
+    ops.status(q.device)
+    want, wl, bound, vmax = _reference(q, cache, lengths, mask, causal, scale)
+    got, gl, ds = out.double(), lse.double(), bound * (2.0 ** -11 + 2.0 ** -20)
+    bf16 = q.dtype == torch.bfloat16
+    empty = torch.isinf(wl)
+    assert torch.equal(torch.isinf(gl), empty) and (got.transpose(1, 2)[empty] == 0).all()
+    tol = (2.0 ** -10 + max(lengths) * 2.0 ** -25 + 2 * ds) * vmax + (2.0 ** -8 if bf16 else 2.0 ** -11) * want.abs()
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() - tol).max())
+    assert (got - want).norm() <= (2.0 ** -9 + (2.0 ** -9 if bf16 else 2.0 ** -12)) * want.norm()
+    err = (gl - wl)[~empty].abs()
+    assert (err <= ds + 2e-5 + 1e-6 * wl[~empty].abs()).all() and err.mean() <= 2.0 ** -10
+    return out, lse
+
+
+FORMATS = list(itertools.product((4, 8), (32, 64, 128)))
+
+
+@pytest.mark.parametrize("bits,group", FORMATS)
+@pytest.mark.parametrize("batch,heads,groups,queries,length", [
+    (4, 8, 1, 381, 100),  # two row tiles, the last row in the middle of a warp, nothing split
+    (2, 8, 1, 439, 767),  # a partial second tile of rows; parts joined by a warp a row
+    (1, 4, 5, 133, 2900),  # 665 rows: a third pair of tiles with 25 of 32 lanes of a warp
+])
+def test_rows_that_end_inside_a_warp(bits, group, batch, heads, groups, queries, length):
+    dev = _dev()
+    lengths = [max(length - 61 * b, 0) for b in range(batch)]
+    c = _filled(200, batch, heads, -(-length // 128) * 128, bits, group, dev, lengths)
+    q = _rows(202, (batch, heads * groups, queries, 128), DT["bf16"], 2.0).to(dev)
+    _check_many(q, c, lengths)
