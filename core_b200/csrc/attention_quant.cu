@@ -26,12 +26,12 @@
 //  * A warp owns 32-token tiles (every fourth of its CTA's) with its own ring of
 //    bulk copies, running maxima and sums: nothing waits for another warp until
 //    the CTA's four results are joined.  The maximum is raised only when a score
-//    passes it by 2^8.
+//    passes it by 2^7.
 //  * A sequence is cut over CTAs when there are few (batch row, KV head) pairs; a
 //    second kernel, set up while the parts run, joins them.  Which kernel takes a
 //    call and into how many parts is decided by modelled times (below).
-//  * Sums, maxima and the LSE are f32.  P is rounded to f16 (at most 2^8, below
-//    2^-24 of the row's largest it vanishes) and so are V's values; scores are not.
+//  * Sums, maxima and the LSE are f32.  P is rounded to f16 (2^7 at the running
+//    maximum; below 2^-32 of the row's largest it vanishes) and so are V's values; scores are not.
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         mx[n][h] = fmaxf(fmaxf(sc[0][n][h], sc[0][n][h + 2]), fmaxf(sc[1][n][h], sc[1][n][h + 2]));
-        raise |= mx[n][h] > m_used[n][h] + kRaise;
+        raise |= mx[n][h] - m_used[n][h] > kRaise;
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          if (v > m_used[n][h] + kRaise) {
+          if (v - m_used[n][h] > kRaise) {
             const float f = ex2_approx(m_used[n][h] - v);
             m_used[n][h] = v;
             l[n][h] *= f;
@@ -437,8 +437,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
     uint32_t pf[2][kNT][2];
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      const float b0 = m_used[n][0] == -INFINITY ? 0.f : m_used[n][0];
-      const float b1 = m_used[n][1] == -INFINITY ? 0.f : m_used[n][1];
+      const float b0 = m_used[n][0] == -INFINITY ? 0.f : m_used[n][0] - kLift;
+      const float b1 = m_used[n][1] == -INFINITY ? 0.f : m_used[n][1] - kLift;
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         const float e0 = ex2_approx(sc[mt][n][0] - b0), e1 = ex2_approx(sc[mt][n][1] - b1);
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) sm_m[w][r] = f[w] * inv;
-    const float lse2 = lt == 0.f ? -INFINITY : m + log2f(lt);
+    const float lse2 = lt == 0.f ? -INFINITY : m + (log2f(lt) - kLift);
     if (row < rows) {
       if (p.n_split > 1) {
         const long long at = ((long long)bh * rows + row) * p.n_split + split;

@@ -10,7 +10,11 @@
 namespace core {
 namespace kvq {
 
-constexpr float kRaise = 8.0f;  // a running maximum is raised when a score passes it by this: P <= 2^8
+// A running maximum is raised when a score passes it by more than kRaise (in powers of
+// two; compared as a difference, which is exact), and P = 2^(S - maximum + kLift): 2^14
+// at most, which leaves f16 room for what rounding adds to maxima above 2^23, down to
+// 2^-25, 2^-32 of a row's largest.  Without the lift a long tail of weights of 2^-25 was lost.
+constexpr float kRaise = 7.0f, kLift = 7.0f;
 
 struct AttnParams {
   const uint8_t* kc;

@@ -34,9 +34,9 @@
 // writing; the rest is the way of S from tensor core to registers and back.
 //
 // Keys and values are rounded to f16 (2^-11; bf16 would lose three more bits),
-// queries stay exact behind a power of two per row, P is f16 at most 2^8, sums and
-// statistics are f32.  The maximum of a row is raised, and O_x rescaled, only when
-// a score passes it by 2^8.
+// queries stay exact behind a power of two per row, P is f16 (2^7 at the running
+// maximum, at most 2^14), sums and statistics are f32.  The maximum of a row is
+// raised, and O_x rescaled, only when a score passes it by 2^7.
 #include <cuda_bf16.h>
 
 #include "attention_quant.cuh"
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
           for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], v[e + 2 * c], v[e + 2 * c + 1]);
         }
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-        const bool raise = mt > m_used + kRaise;
+        const bool raise = mt - m_used > kRaise;
         // O_x holds every earlier tile, and P_x may be written again, once the last
         // P V has landed
         auto last_pv = [&]() -> bool {
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
           }
           if (raise) m_used = mt;
         }
-        const float neg = m_used == -INFINITY ? 0.f : -m_used;
+        const float neg = m_used == -INFINITY ? 0.f : kLift - m_used;
         const unsigned long long neg2 = f2_pack(neg, neg);
         unsigned long long acc = 0ull;
 #pragma unroll
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       if (ok) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that saw no token: output 0, LSE -inf
-        const float lse2 = l == 0.f ? -INFINITY : m_used + log2f(l);
+        const float lse2 = l == 0.f ? -INFINITY : m_used + (log2f(l) - kLift);
         const long long part = ((long long)bh * rows + row) * p.n_split + split;
         const int Hq = p.Hkv * p.G;
         float* of = p.n_split > 1 ? p.part_o + part * kD : nullptr;

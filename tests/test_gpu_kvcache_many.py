@@ -83,3 +83,47 @@ def test_rows_that_end_inside_a_warp(bits, group, batch, heads, groups, queries,
     c = _filled(200, batch, heads, -(-length // 128) * 128, bits, group, dev, lengths)
     q = _rows(202, (batch, heads * groups, queries, 128), DT["bf16"], 2.0).to(dev)
     _check_many(q, c, lengths)
+
+
+@pytest.mark.parametrize("bits", (4, 8))
+@pytest.mark.parametrize("heads,queries,length", [(160, 48, 16384), (600, 1, 8192)], ids=["many", "few"])
+def test_long_flat_tail_behind_a_large_score(bits, heads, queries, length):
+    """One token whose weight is 2^25.6 times each of the others', with value 0 where
+    theirs is 1: the output is the others' share.  Each weight is rounded at 2^-25 of f16's
+    range, at 2^7 for the largest: off by 2^-32 of 2^-25.6, so by less than 2^-6 of itself."""
+    from core_b200 import ops
+    from core_b200.kvcache import QuantizedKV
+    dev = _dev()
+    c = QuantizedKV.empty(1, heads, length, bits=bits, group=128, device=dev)
+    c.k_codes.zero_(), c.v_codes.zero_(), c.k_meta.zero_(), c.v_meta.zero_()
+    c.k_meta[:, :, 0, :, 1] = 25.6 / 128
+    c.v_meta[:, :, 1:, :, 1] = 1.0
+    q = torch.ones(1, heads, queries, 128, dtype=torch.bfloat16, device=dev)
+    scale = 0.6931471805599453
+    out, lse = ops.attention_quantized(q, c, length, causal=False, softmax_scale=scale)
+    s0 = torch.tensor(25.6 / 128).half().double() * 128 * scale
+    share = (length - 1) * torch.exp(-s0) / (1 + (length - 1) * torch.exp(-s0))
+    assert ((out.double() / share - 1).abs() <= 2.0 ** -6 + 2.0 ** -8).all(), float(out.max()) / float(share)
+    assert ((lse.double().cpu() - s0 - torch.log1p((length - 1) * torch.exp(-s0))).abs() < 1e-4).all()
+
+
+@pytest.mark.parametrize("heads,queries", [(160, 48), (2, 1)], ids=["many", "few"])
+@pytest.mark.parametrize("power", (20, 23, 24, 25, 26))
+def test_scores_whose_last_place_is_whole_numbers(power, heads, queries):
+    """Scores of 2^power and a few units that rise along the sequence: P stays within f16
+    although the maxima are rounded.  All values are 1, so the output is 1."""
+    from core_b200 import ops
+    from core_b200.kvcache import QuantizedKV
+    dev = _dev()
+    n = 4096
+    c = QuantizedKV.empty(1, heads, n, bits=8, group=32, device=dev)
+    c.k_codes.zero_(), c.v_codes.zero_(), c.k_meta.zero_(), c.v_meta.zero_()
+    c.k_meta[:, :, :, 0, 1] = 256.0
+    c.k_meta[:, :, :, 1, 1] = torch.linspace(0, 64, n, device=dev)
+    c.v_meta[..., 1] = 1.0
+    q = torch.zeros(1, heads, queries, 128, dtype=torch.float16, device=dev)
+    q[..., 0], q[..., 32] = 2.0 ** (power - 8 - 8), 2.0 ** -8
+    scale = 0.6931471805599453 * 2.0 ** 8
+    out, lse = ops.attention_quantized(q, c, n, causal=False, softmax_scale=scale)
+    assert (out == 1).all()
+    assert ((lse / 0.6931471805599453 / 2.0 ** power - 1).abs() < 1e-4).all()
