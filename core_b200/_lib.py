@@ -84,6 +84,16 @@ class CoreKvq(ctypes.Structure):
     ]
 
 
+class CoreKvqPlan(ctypes.Structure):
+    _fields_ = [
+        ("row_tile", ctypes.c_int32),
+        ("ctas_per_sm", ctypes.c_int32),
+        ("parts", ctypes.c_int32),
+        ("join_rows", ctypes.c_int32),
+        ("f16_keys", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _F = ctypes.c_float
@@ -139,6 +149,7 @@ SIGNATURES = {
     "core_kvq_quantize": (ctypes.c_int, [_Q, _I, _P, _P, _P, _P, _I, _I, _P, _P, _I, _P, _P]),
     "core_kvq_dequantize": (ctypes.c_int, [_Q, _I, _I, _P, _P, _I, _P, _P, _P]),
     "core_kvq_attention_workspace_bytes": (_S, [_Q, _I, _I, _I]),
+    "core_kvq_attention_plan": (ctypes.c_int, [_Q, _I, _I, _I, ctypes.POINTER(CoreKvqPlan)]),
     "core_kvq_attention": (ctypes.c_int, [_Q, _I, _I, _I, _P, _P, _P, _I, _P, ctypes.c_int64, _I,
                                           _F, _P, _P, _P, _S, _P]),
     "core_compress_layer_workspace_bytes": (_S, [_D, _I, _I]),

@@ -742,6 +742,7 @@ double many_us(int bits, long long units, long long rows, int tiles, int n) {
 struct Plan {
   bool many;
   int nt, ctas, n_rt, n_split;  // few rows: tiles of 8 rows a CTA, CTAs an SM
+  bool join_rows;               // the parts are joined by a warp a row, not a CTA
 };
 
 // Which kernel takes the call, and into how many parts it cuts the sequences.
@@ -773,7 +774,7 @@ Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len) {
         const double us = few_us(bits, ctas, nt, heads * n_rt, few_tiles, n);
         if (r.n_split == 0 || us < best) {
           best = us;
-          r = {false, nt, ctas, n_rt, n};
+          r = {false, nt, ctas, n_rt, n, false};
         }
       }
     }
@@ -787,7 +788,7 @@ Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len) {
     const double us = many_us(bits, many_units, rows, many_tiles, n);
     if (us < best) {
       best = us;
-      r = {true, 0, 1, many_rt, n};
+      r = {true, 0, 1, many_rt, n, false};
     }
   }
   return r;
@@ -805,6 +806,9 @@ Plan plan(int bits, int B, int Hkv, long long rows, int max_len) {
   for (int i = 0; i < 6; ++i) same = same && key[i] == last.key[i];
   if (!same) {
     last.plan = make_plan(bits, B, Hkv, rows, max_len);
+    // A warp a row where rows are many for their parts, else a CTA a row: 16384 rows of
+    // 2 parts 171 -> 153 us with the attention itself, 2048 rows of 8 parts 31.2 -> 34.9.
+    last.plan.join_rows = rows * B * Hkv > (long long)sm_count() * 8 * last.plan.n_split;
     for (int i = 0; i < 6; ++i) last.key[i] = key[i];
   }
   return last.plan;
@@ -863,6 +867,28 @@ extern "C" size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, in
   float *a, *b;
   carve_parts(z, pl.n_split, rows * cache->batch * cache->n_kv_heads, &a, &b);
   return z.used;
+}
+
+extern "C" int core_kvq_attention_plan(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries,
+                                       int32_t max_length, core_kvq_plan_t* out) {
+  const char* fn = "core_kvq_attention_plan";
+  int rc = check_kvq(cache, fn);
+  if (rc != CORE_OK) return rc;
+  const std::string f(fn);
+  if (out == nullptr) return set_error(CORE_ERR_INVALID_ARG, f + ": NULL argument");
+  if (n_q_heads <= 0 || n_queries <= 0 || n_q_heads % cache->n_kv_heads != 0)
+    return set_error(CORE_ERR_INVALID_ARG, f + ": bad query dimensions");
+  if (max_length < 0 || max_length > cache->capacity)
+    return set_error(CORE_ERR_INVALID_ARG, f + ": max_length outside the cache's capacity");
+  const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
+  if (rows > INT_MAX / 2) return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
+  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length);
+  out->row_tile = pl.many ? kvq::kManyRows : 8 * pl.nt;
+  out->ctas_per_sm = pl.ctas;
+  out->parts = pl.n_split;
+  out->join_rows = pl.n_split > 1 && pl.join_rows;
+  out->f16_keys = pl.many;
+  return CORE_OK;
 }
 
 extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_t n_q_heads, int32_t n_queries,
@@ -924,11 +950,8 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
   carve_parts(c, pl.n_split, rows * p.B * p.Hkv, &p.part_o, &p.part_lse);
   if (c.overflow) return set_error(CORE_ERR_WORKSPACE, f + ": workspace too small");
   const long long blocks = (long long)p.B * p.Hkv * pl.n_rt * pl.n_split;
-  // A warp a row where rows are many for their parts, else a CTA a row: 16384 rows of
-  // 2 parts 171 -> 153 us with the attention itself, 2048 rows of 8 parts 31.2 -> 34.9.
   const long long all_rows = rows * p.B * p.Hkv;
-  const bool join_rows = all_rows > (long long)sm_count() * 8 * pl.n_split;
-  const long long join_blocks = join_rows ? (all_rows + 3) / 4 : all_rows;
+  const long long join_blocks = pl.join_rows ? (all_rows + 3) / 4 : all_rows;
   if (blocks > INT_MAX || join_blocks > INT_MAX)
     return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -956,8 +979,8 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
     cfg.stream = s;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, join_rows ? kvq::attn_join_rows_kernel : kvq::attn_join_kernel, p, pl.many ? kvq::kManyRows : 8 * pl.nt,
-                           pl.many ? kvq::kManyTok : kvq::kTok);
+    e = cudaLaunchKernelEx(&cfg, pl.join_rows ? kvq::attn_join_rows_kernel : kvq::attn_join_kernel, p,
+                           pl.many ? kvq::kManyRows : 8 * pl.nt, pl.many ? kvq::kManyTok : kvq::kTok);
     if (e != cudaSuccess) return cuda_error(e, "attn_join_kernel launch");
   }
   return CORE_OK;

@@ -355,6 +355,18 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     return out, lse
 
 
+def attention_quantized_plan(cache, n_q_heads: int, n_queries: int, max_length: int) -> dict:
+    """How :func:`attention_quantized` carries out a call of these sizes: ``row_tile``
+    (query rows of a KV head a CTA takes: 8, 16, 24, or 256 on tcgen05), ``ctas_per_sm``,
+    ``parts`` (CTAs a sequence is cut over), ``join_rows`` (parts joined by a warp a
+    row) and ``f16_keys`` (keys rounded to f16; otherwise scores are exact to f32)."""
+    plan = _lib.CoreKvqPlan()
+    check(_lib.load().core_kvq_attention_plan(cache.handle, n_q_heads, n_queries, max_length,
+                                              ctypes.byref(plan)))
+    return {name: bool(getattr(plan, name)) if name in ("join_rows", "f16_keys") else getattr(plan, name)
+            for name, _ in plan._fields_}
+
+
 def split_bf16(w: torch.Tensor, terms: int) -> torch.Tensor:
     """f32 -> (terms, *w.shape) bf16 whose sum reproduces w (hi, mid, lo)."""
     _require_cuda(w)

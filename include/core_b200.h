@@ -510,6 +510,17 @@ int core_kvq_dequantize(const core_kvq_t* cache, int32_t dtype, int32_t n_rows, 
  * whatever their bytes hold. */
 size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries,
                                           int32_t max_length);
+
+/* How a call of core_kvq_attention with these sizes is carried out; launches nothing. */
+typedef struct core_kvq_plan {
+  int32_t row_tile;    /* query rows of a KV head that a CTA takes: 8, 16, 24, or 256 on tcgen05 */
+  int32_t ctas_per_sm; /* that the kernel was built for */
+  int32_t parts;       /* CTAs that a sequence is cut over */
+  int32_t join_rows;   /* 1: the parts are joined by a warp a row, 0: by a CTA a row, or not cut */
+  int32_t f16_keys;    /* 1: n s + z of the keys is rounded to f16, 0: scores are exact to f32 */
+} core_kvq_plan_t;
+int core_kvq_attention_plan(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries, int32_t max_length,
+                            core_kvq_plan_t* plan);
 int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_t n_q_heads, int32_t n_queries,
                        const void* q, const int64_t* q_strides, const int32_t* lengths,
                        int32_t max_length, const uint8_t* key_mask, int64_t mask_stride, int32_t causal,

@@ -1,7 +1,9 @@
-"""Attention over the quantised cache at sizes that the many-row kernel takes, every
-value and LSE against a plain f64 computation.
+"""Attention over the quantised cache, every value and LSE against a plain f64
+computation, at sizes that reach each kernel, tile and join; the plan of each call is
+asked for, so that a change of the plan cannot leave one untested.
 
-Tolerances.  K, V and P are rounded to f16 (relative 2^-11 at most, 0.41 of it in the
+Tolerances, of the kernel that the plan names.  The few-row kernels' scores are off by
+2^-20 scale sum|q||k| (f32 sums of exact products).  On tcgen05 K, V and P are rounded to f16 (relative 2^-11 at most, 0.41 of it in the
 mean square).  A score is then off by 2^-11 scale sum|q||k| at most, which moves the
 output by twice that times max|v| beside P's and V's 2^-10 max|v|, and the LSE by as much.
 Each weight and value is off by an independent relative error, so the error's norm stands
@@ -49,14 +51,18 @@ def _reference(q, cache, lengths, mask, causal, scale):
     return out, lse, bound, vmax
 
 
-def _check_many(q, cache, lengths, *, mask=None, causal=True, scale=128 ** -0.5):
+def _check_plan(q, cache, lengths, plan, *, mask=None, causal=True, scale=128 ** -0.5):
+    """``plan``: what ops.attention_quantized_plan has to say of the call."""
     from core_b200 import ops
+    got = ops.attention_quantized_plan(cache, q.shape[1], q.shape[2], max(lengths))
+    assert {k: got[k] > 1 if k == "parts" else got[k] for k in plan} == plan, got
     at = torch.tensor(lengths, dtype=torch.int32, device=q.device)
     out, lse = ops.attention_quantized(q, cache, at, max_length=max(lengths), key_mask=mask, causal=causal,
                                        softmax_scale=scale)
     ops.status(q.device)
     want, wl, bound, vmax = _reference(q, cache, lengths, mask, causal, scale)
-    got, gl, ds = out.double(), lse.double(), bound * (2.0 ** -11 + 2.0 ** -20)
+    ds = bound * (2.0 ** -20 + (2.0 ** -11 if got["f16_keys"] else 0.0))
+    got, gl = out.double(), lse.double()
     bf16 = q.dtype == torch.bfloat16
     empty = torch.isinf(wl)
     assert torch.equal(torch.isinf(gl), empty) and (got.transpose(1, 2)[empty] == 0).all()
@@ -68,21 +74,74 @@ def _check_many(q, cache, lengths, *, mask=None, causal=True, scale=128 ** -0.5)
     return out, lse
 
 
+MANY = dict(row_tile=256, f16_keys=True)
+ONE, CTA, WARP = dict(parts=False), dict(parts=True, join_rows=False), dict(parts=True, join_rows=True)
 FORMATS = list(itertools.product((4, 8), (32, 64, 128)))
 
 
 @pytest.mark.parametrize("bits,group", FORMATS)
-@pytest.mark.parametrize("batch,heads,groups,queries,length", [
-    (4, 8, 1, 381, 100),  # two row tiles, the last row in the middle of a warp, nothing split
-    (2, 8, 1, 439, 767),  # a partial second tile of rows; parts joined by a warp a row
-    (1, 4, 5, 133, 2900),  # 665 rows: a third pair of tiles with 25 of 32 lanes of a warp
+@pytest.mark.parametrize("batch,heads,groups,queries,length,plan", [
+    (4, 8, 1, 381, 100, ONE),  # two row tiles, the last row in the middle of a warp
+    (2, 8, 1, 439, 767, WARP),  # a partial second tile of rows
+    (1, 4, 5, 133, 2900, CTA),  # 665 rows: a third pair of tiles with 25 of 32 lanes of a warp
 ])
-def test_rows_that_end_inside_a_warp(bits, group, batch, heads, groups, queries, length):
+def test_rows_that_end_inside_a_warp(bits, group, batch, heads, groups, queries, length, plan):
     dev = _dev()
     lengths = [max(length - 61 * b, 0) for b in range(batch)]
     c = _filled(200, batch, heads, -(-length // 128) * 128, bits, group, dev, lengths)
     q = _rows(202, (batch, heads * groups, queries, 128), DT["bf16"], 2.0).to(dev)
-    _check_many(q, c, lengths)
+    _check_plan(q, c, lengths, dict(MANY, **plan))
+
+
+@pytest.mark.parametrize("bits,group", FORMATS)
+@pytest.mark.parametrize("batch,heads,groups,queries,length,plan", [
+    (16, 8, 3, 17, 100, ONE), (1, 8, 11, 11, 3308, CTA), (8, 8, 1, 79, 767, WARP),  # one row tile
+    (8, 8, 11, 17, 100, ONE), (1, 8, 6, 27, 3970, CTA), (4, 8, 3, 83, 767, WARP),  # two
+])
+def test_row_tiles_masks_and_lengths(bits, group, batch, heads, groups, queries, length, plan):
+    """One and two row tiles, alone and cut into parts that either join takes: ragged and
+    empty sequences, causal and not, and masks with NaN and infinities behind them."""
+    from core_b200 import ops
+    dev = _dev()
+    lengths = [length if b % 3 == 0 else 0 if b % 5 == 4 else length * (b + 1) // (batch + 1) for b in range(batch)]
+    cap = -(-length // 128) * 128
+    c = _filled(210, batch, heads, cap, bits, group, dev, lengths)
+    q = _rows(212, (batch, heads * groups, queries, 128), DT["f16"], 2.0).to(dev)
+    plan = dict(MANY, **plan)
+    _check_plan(q, c, lengths, plan)
+    _check_plan(q.to(torch.bfloat16), c, lengths, plan, causal=False, scale=0.06)
+    mask = torch.rand(batch, cap, generator=torch.Generator().manual_seed(213)) < 0.5
+    mask[0, :length // 2] = False
+    mask[batch // 2, :length // 3] = True
+    if batch > 2:
+        mask[2] = False
+    k, v = _rows(214, (batch, heads, length, 128), DT["bf16"], 6.0), _rows(215, (batch, heads, length, 128), DT["bf16"])
+    hidden = ~mask[:, None, :length, None].expand_as(k)
+    k[hidden], v[hidden] = float("nan"), float("inf")
+    v[:, 1:][hidden[:, 1:]] = float("nan")
+    ops.kv_quantize(k.to(dev), v.to(dev), c, 0)
+    _check_plan(q, c, [length] * batch, plan, mask=mask.to(dev))
+    _check_plan(q, c, lengths, plan, mask=mask.to(dev), causal=False)
+
+
+@pytest.mark.parametrize("bits,group", FORMATS)
+@pytest.mark.parametrize("heads,groups,queries,length,plan", [
+    (50, 4, 5, 2400, dict(row_tile=24, **CTA)), (50, 6, 4, 2400, dict(row_tile=24, **CTA)),
+    (113, 4, 6, 2000, dict(row_tile=24, **WARP)), (1, 1, 1, 492, dict(row_tile=8, ctas_per_sm=3, **CTA)),
+    (64, 1, 1, 3096, dict(row_tile=8, **CTA)), (64, 8, 1, 3096, dict(row_tile=8, **CTA)),
+    (1, 4, 4, 3000, dict(row_tile=16, **CTA)),
+])
+def test_few_rows_tiles_and_joins(bits, group, heads, groups, queries, length, plan):
+    """8, 16 and 24 rows a CTA whose parts are joined, in every format."""
+    dev = _dev()
+    c = _filled(220, 1, heads, -(-length // 128) * 128, bits, group, dev, [length])
+    q = _rows(222, (1, heads * groups, queries, 128), DT["bf16"], 2.0).to(dev)
+    plan = dict(plan, f16_keys=False)
+    if (heads, bits) == (64, 4):
+        plan["ctas_per_sm"] = 4
+    _check_plan(q, c, [length], plan)
+    mask = torch.rand(1, length, generator=torch.Generator().manual_seed(223)).to(dev) > 0.3
+    _check_plan(q.half(), c, [length], plan, mask=mask)
 
 
 @pytest.mark.parametrize("bits", (4, 8))

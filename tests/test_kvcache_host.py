@@ -77,3 +77,31 @@ def test_operators_run_with_the_cache_device_current(monkeypatch):
         with pytest.raises(TypeError, match="attention_quantized takes"):
             ops.attention_quantized(rows, cache, 4)
     assert now == [0] and seen == [1, 1, 1]
+
+
+def test_attention_plan_on_host():
+    """The plan can be asked for without a GPU: few rows keep the keys exact, many long rows go to tcgen05,
+    bad sizes are refused."""
+    import types
+
+    import pytest
+
+    from core_b200 import ops
+
+    def plan(hq, nq, n, heads=8, cap=1 << 20, bits=4):
+        kvq = _lib.CoreKvq(256, 256, 256, 256, 1, heads, cap, bits, 64)
+        return ops.attention_quantized_plan(types.SimpleNamespace(handle=ctypes.byref(kvq)), hq, nq, n)
+
+    for nq in (1, 2, 3, 4, 8):
+        p = plan(32, nq, 131072)
+        assert not p["f16_keys"] and p["row_tile"] == min(8 * -(-4 * nq // 8), 24 if p["row_tile"] == 24 else 16)
+    assert plan(8, 1, 131072, heads=1)["parts"] > 1  # the host counts one SM
+    assert plan(8, 1, 0)["parts"] == 1
+    p = plan(32, 2048, 16384)
+    assert p["f16_keys"] and p["row_tile"] == 256
+    for bad in (lambda: plan(12, 1, 5), lambda: plan(8, 0, 5), lambda: plan(8, 1, -1), lambda: plan(8, 1, 129, cap=128),
+                lambda: plan(8, 1, 5, bits=3)):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert _lib.load().core_kvq_attention_plan(ctypes.byref(_lib.CoreKvq(256, 256, 256, 256, 1, 8, 128, 4, 64)),
+                                               8, 1, 5, None) == -1
