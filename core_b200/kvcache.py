@@ -19,6 +19,12 @@ from . import _lib, ops
 CAPACITY_STEP = 128
 
 
+def _normal_tensors():
+    """A cache outlives the forward that creates it: its tensors are changed in place
+    later, which those made under inference_mode do not allow outside of it."""
+    return torch.inference_mode(False)
+
+
 class QuantizedKV:
     """One layer's K and V in 4 or 8 bits.
 
@@ -76,15 +82,17 @@ class QuantizedKV:
         cap = -(-int(capacity) // CAPACITY_STEP) * CAPACITY_STEP
         codes = (batch, n_kv_heads, cap, 16 * bits)
         meta = (batch, n_kv_heads, cap, 128 // group, 2)
-        return cls(torch.empty(codes, dtype=torch.uint8, device=device),
-                   torch.empty(meta, dtype=torch.float16, device=device),
-                   torch.empty(codes, dtype=torch.uint8, device=device),
-                   torch.empty(meta, dtype=torch.float16, device=device))
+        with _normal_tensors():
+            return cls(torch.empty(codes, dtype=torch.uint8, device=device),
+                       torch.empty(meta, dtype=torch.float16, device=device),
+                       torch.empty(codes, dtype=torch.uint8, device=device),
+                       torch.empty(meta, dtype=torch.float16, device=device))
 
     @property
     def lengths(self) -> torch.Tensor:
         if self._lengths is None:
-            self._lengths = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
+            with _normal_tensors():
+                self._lengths = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
         return self._lengths
 
     @property
@@ -102,17 +110,19 @@ class QuantizedKV:
             return
         used = -(-self.max_length // CAPACITY_STEP) * CAPACITY_STEP
         new = []
-        for t in self.buffers:
-            n = t.new_empty((*t.shape[:2], cap, *t.shape[3:]))
-            n[:, :, :used] = t[:, :, :used]
-            new.append(n)
+        with _normal_tensors():
+            for t in self.buffers:
+                n = t.new_empty((*t.shape[:2], cap, *t.shape[3:]))
+                n[:, :, :used] = t[:, :, :used]
+                new.append(n)
         self._take(new)
 
     def select(self, rows: torch.Tensor) -> None:
         """Keep the sequences ``rows`` (an index along the batch, repeats allowed)."""
-        rows = rows.to(self.device, torch.int64)
-        lengths = self.lengths.index_select(0, rows)
-        self._take([t.index_select(0, rows) for t in self.buffers])
+        with _normal_tensors():
+            rows = rows.to(self.device, torch.int64)
+            lengths = self.lengths.index_select(0, rows)
+            self._take([t.index_select(0, rows) for t in self.buffers])
         self._lengths = lengths
 
     def crop(self, length: int) -> None:

@@ -152,3 +152,19 @@ def test_refuses_other_head_dims():
         QuantizedCacheLayer().update(torch.zeros(1, 1, 2, 64, device=dev), torch.zeros(1, 1, 2, 64, device=dev))
     with pytest.raises(ValueError, match="bits"):
         QuantizedCacheLayer(bits=3)
+
+
+def test_prompt_under_inference_mode_decoding_under_no_grad():
+    from core_b200.hf_cache import quantized_cache
+    dev = _dev()
+    ids = torch.randint(0, 97, (1, 60), generator=torch.Generator().manual_seed(6)).to(dev)
+    model = _model(dev, "core_b200")
+    want = _steps(model, quantized_cache(model.config), ids, pieces=(1, 1, 3))
+    cache = quantized_cache(model.config)
+    with torch.inference_mode():
+        model(ids[:, :55], past_key_values=cache)
+    with torch.no_grad():
+        got = [model(ids[:, a:b], past_key_values=cache).logits for a, b in ((55, 56), (56, 57), (57, 60))]
+        cache.crop(40)
+        cache.reset()
+    assert torch.equal(torch.cat(got, 1).float(), want)

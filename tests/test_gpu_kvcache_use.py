@@ -1,0 +1,45 @@
+"""The quantised cache's objects in use: modes of autograd, growth, selection, what a
+press keeps, and calls that used to mislead."""
+
+import pytest
+import torch
+
+from test_gpu_kvcache import _dev, _rows
+
+pytestmark = pytest.mark.gpu
+
+
+def _cache(dev, B=2, H=2, cap=256, n=60, bits=4, group=32, seed=300):
+    """(cache with n tokens, its keys, its values)."""
+    from core_b200.kvcache import QuantizedKV
+    c = QuantizedKV.empty(B, H, cap, bits=bits, group=group, device=dev)
+    k = _rows(seed, (B, H, n, 128), torch.bfloat16, 6.0).to(dev)
+    v = _rows(seed + 1, (B, H, n, 128), torch.bfloat16).to(dev)
+    c.append(k, v)
+    return c, k, v
+
+
+def test_filled_under_inference_mode_used_under_no_grad():
+    """A prompt under inference_mode, then decoding, selecting, growing, cropping and
+    resetting outside of it, as transformers' own layers accept."""
+    dev = _dev()
+    with torch.inference_mode():
+        c, k, v = _cache(dev)
+        c.select(torch.tensor([1, 0], device=dev))
+        c.reserve(300)
+    want = c.read()
+    with torch.no_grad():
+        c.append(k[:, :, :1].clone(), v[:, :, :1].clone())
+        assert c.lengths.tolist() == [61, 61]
+        c.select(torch.tensor([1, 0]))
+        c.reserve(500)
+        assert torch.equal(c.read()[0][:, :, :60], want[0][[1, 0]])
+        c.k_codes[:, :, -1].zero_()
+        c.crop(30)
+        assert c.lengths.tolist() == [30, 30]
+    c.append(k[:, :, :1].clone(), v[:, :, :1].clone())
+    assert c.lengths.tolist() == [31, 31]
+    with torch.inference_mode():
+        c.append(k[:, :, :1], v[:, :, :1])
+    c.reset()
+    assert c.lengths.tolist() == [0, 0]
