@@ -104,16 +104,16 @@ class QuantizedKV:
         return sum(t.numel() * t.element_size() for t in self.buffers)
 
     def reserve(self, capacity: int) -> None:
-        """Room for ``capacity`` tokens a sequence: larger buffers with the same rows."""
+        """Room for ``capacity`` tokens a sequence: larger buffers with the same rows,
+        those beyond ``max_length`` among them (written at explicit places)."""
         cap = -(-int(capacity) // CAPACITY_STEP) * CAPACITY_STEP
         if cap <= self.capacity:
             return
-        used = -(-self.max_length // CAPACITY_STEP) * CAPACITY_STEP
         new = []
         with _normal_tensors():
             for t in self.buffers:
                 n = t.new_empty((*t.shape[:2], cap, *t.shape[3:]))
-                n[:, :, :used] = t[:, :, :used]
+                n[:, :, :self.capacity] = t
                 new.append(n)
         self._take(new)
 

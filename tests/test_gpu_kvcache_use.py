@@ -43,3 +43,18 @@ def test_filled_under_inference_mode_used_under_no_grad():
         c.append(k[:, :, :1], v[:, :, :1])
     c.reset()
     assert c.lengths.tolist() == [0, 0]
+
+
+def test_reserve_keeps_rows_written_at_explicit_places():
+    """A cache around filled buffers, or one written with ops.kv_quantize, has rows that
+    its lengths do not count."""
+    from core_b200 import ops
+    from core_b200.kvcache import QuantizedKV
+    dev = _dev()
+    c, k, v = _cache(dev, n=200)
+    want = ops.kv_dequantize(c, count=200)
+    w = QuantizedKV(*c.buffers)
+    w.reserve(900)
+    assert w.capacity == 1024
+    got = ops.kv_dequantize(w, count=200)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
