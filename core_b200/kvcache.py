@@ -149,17 +149,20 @@ class QuantizedKV:
                counts: torch.Tensor | None = None) -> None:
         """Quantise rows (B, Hkv, T, 128) behind each sequence's tokens.  ``index``
         (B, n) picks source rows instead; ``counts`` (B,) writes only the first
-        counts[b] of them."""
+        counts[b] of them.  A source row out of range is skipped and reported by
+        ``ops.status``; the sequence then ends before it.  ``max_length`` grows by n
+        whatever ``counts`` says (it is not read back); ``crop`` lowers it."""
         n = keys.shape[2] if index is None else index.shape[1]
         if n == 0:
             return
         if self.max_length + n > self.capacity:
             raise ValueError(f"{self.max_length} + {n} tokens exceed the cache's capacity {self.capacity}")
         ops.kv_quantize(keys, values, self, self.lengths, index=index, counts=counts)
-        if counts is None:
-            self.lengths.add_(n)
-        else:
-            self.lengths.add_(counts.to(device=self.device, dtype=torch.int32).clamp(0, n))
+        added = n if counts is None else counts.clamp(0, n)
+        if index is not None:
+            there = ((index >= 0) & (index < keys.shape[2])).cumprod(1).sum(1, dtype=torch.int32)
+            added = there if counts is None else torch.minimum(there, added)
+        self.lengths.add_(added)
         self.max_length += n
 
     def read(self, *, index: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16):

@@ -58,3 +58,23 @@ def test_reserve_keeps_rows_written_at_explicit_places():
     assert w.capacity == 1024
     got = ops.kv_dequantize(w, count=200)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_append_counts_only_rows_that_were_written():
+    """A source row out of range is skipped and reported: the sequence ends before it, so
+    that no slot that was never written is attended to."""
+    from core_b200 import ops
+    from core_b200._lib import CoreError
+    dev = _dev()
+    c, k, v = _cache(dev, B=4, n=10)
+    index = torch.tensor([[3, 4, 5, 6], [3, 60, 5, 6], [-1, 4, 5, 6], [0, 1, 2, 99]], device=dev)
+    counts = torch.tensor([4, 4, 4, 2], dtype=torch.int32, device=dev)
+    for idx in (index, index.int()):
+        c.append(k, v, index=idx, counts=counts)
+        with pytest.raises(CoreError, match="where=1402"):
+            ops.status(dev)
+        assert c.lengths.tolist() == [14, 11, 10, 12]
+        c.crop(10)
+    c.append(k, v, index=index[:1].expand(4, -1))
+    assert c.lengths.tolist() == [14] * 4
+    ops.status(dev)
