@@ -277,6 +277,8 @@ def kv_dequantize(cache, *, start=0, count: int | None = None, index: torch.Tens
     if index is not None:
         index = _row_index(index, cache, "index")
         n, idx = index.shape[1], index.data_ptr()
+        if isinstance(start, torch.Tensor) or start != 0 or count not in (None, n):
+            raise ValueError("kv_dequantize reads the slots of index: no start, and no other count")
     else:
         if count is None or count < 0:
             raise ValueError("kv_dequantize needs index, or a count of slots")

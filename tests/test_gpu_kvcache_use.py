@@ -78,3 +78,15 @@ def test_append_counts_only_rows_that_were_written():
     c.append(k, v, index=index[:1].expand(4, -1))
     assert c.lengths.tolist() == [14] * 4
     ops.status(dev)
+
+
+def test_reading_picked_rows_takes_no_start_and_no_other_count():
+    from core_b200 import ops
+    dev = _dev()
+    c, _, _ = _cache(dev)
+    index = torch.tensor([[3, 4, 5], [6, 7, 8]], device=dev)
+    want = ops.kv_dequantize(c, index=index)
+    assert torch.equal(ops.kv_dequantize(c, index=index, count=3)[1], want[1])
+    for bad in (dict(start=1), dict(start=torch.zeros(2, dtype=torch.int32, device=dev)), dict(count=2)):
+        with pytest.raises(ValueError):
+            ops.kv_dequantize(c, index=index, **bad)
