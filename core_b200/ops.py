@@ -196,10 +196,18 @@ def _aligned_rows(t: torch.Tensor):
     return t, _I64X3(s0, s1, s2)
 
 
+def _int32(value, name: str) -> int:
+    """A host number that the C entry takes in 32 bits: ctypes would cut it off."""
+    n = int(value)
+    if not -2 ** 31 <= n < 2 ** 31:
+        raise ValueError(f"{name} does not fit 32 bits: {n}")
+    return n
+
+
 def _per_sequence(value, cache, name: str):
     """(pointer to (B,) int32 on the device, scalar) of an int or a tensor."""
     if not isinstance(value, torch.Tensor):
-        return None, int(value)
+        return None, _int32(value, name)
     if value.shape != (cache.batch,) or value.dtype is not torch.int32 or not value.is_contiguous():
         raise ValueError(f"{name} must be an int or a contiguous (B,) int32 tensor")
     if value.get_device() != cache.index:
@@ -282,7 +290,7 @@ def kv_dequantize(cache, *, start=0, count: int | None = None, index: torch.Tens
     else:
         if count is None or count < 0:
             raise ValueError("kv_dequantize needs index, or a count of slots")
-        n = int(count)
+        n = _int32(count, "count")
         at, at0 = _per_sequence(start, cache, "start")
     k = cache.k_meta.new_empty((cache.batch, cache.n_kv_heads, n, HEAD_DIM), dtype=dtype)
     v = torch.empty_like(k)
@@ -324,7 +332,7 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     B, Hq, Lq, _ = shape
     at, n = _per_sequence(lengths, cache, "lengths")
     if at is not None:
-        n = cache.capacity if max_length is None else int(max_length)
+        n = cache.capacity if max_length is None else _int32(max_length, "max_length")
     mask, mask_stride = None, 0
     if key_mask is not None:
         if (key_mask.dim() != 2 or key_mask.shape[0] != B or key_mask.shape[1] < n
@@ -363,8 +371,9 @@ def attention_quantized_plan(cache, n_q_heads: int, n_queries: int, max_length: 
     ``parts`` (CTAs a sequence is cut over), ``join_rows`` (parts joined by a warp a
     row) and ``f16_keys`` (keys rounded to f16; otherwise scores are exact to f32)."""
     plan = _lib.CoreKvqPlan()
-    check(_lib.load().core_kvq_attention_plan(cache.handle, n_q_heads, n_queries, max_length,
-                                              ctypes.byref(plan)))
+    check(_lib.load().core_kvq_attention_plan(
+        cache.handle, _int32(n_q_heads, "n_q_heads"), _int32(n_queries, "n_queries"),
+        _int32(max_length, "max_length"), ctypes.byref(plan)))
     return {name: bool(getattr(plan, name)) if name in ("join_rows", "f16_keys") else getattr(plan, name)
             for name, _ in plan._fields_}
 

@@ -90,3 +90,21 @@ def test_reading_picked_rows_takes_no_start_and_no_other_count():
     for bad in (dict(start=1), dict(start=torch.zeros(2, dtype=torch.int32, device=dev)), dict(count=2)):
         with pytest.raises(ValueError):
             ops.kv_dequantize(c, index=index, **bad)
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    """They would wrap to other rows at the C boundary."""
+    from core_b200 import ops
+    dev = _dev()
+    c, k, v = _cache(dev)
+    before = [t.clone() for t in c.buffers]
+    q = _rows(310, (2, 4, 1, 128), torch.bfloat16).to(dev)
+    at = torch.full((2,), 60, dtype=torch.int32, device=dev)
+    for far in (2 ** 32, 2 ** 32 + 3, -2 ** 32, 2 ** 31):
+        for call in (lambda: ops.kv_quantize(k, v, c, far), lambda: ops.kv_dequantize(c, start=far, count=3),
+                     lambda: ops.attention_quantized(q, c, far),
+                     lambda: ops.attention_quantized(q, c, at, max_length=far),
+                     lambda: ops.attention_quantized_plan(c, 4, 1, far)):
+            with pytest.raises((ValueError, RuntimeError)):
+                call()
+    assert all(torch.equal(a, b) for a, b in zip(before, c.buffers))
