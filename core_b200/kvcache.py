@@ -118,9 +118,12 @@ class QuantizedKV:
         self._take(new)
 
     def select(self, rows: torch.Tensor) -> None:
-        """Keep the sequences ``rows`` (an index along the batch, repeats allowed)."""
+        """Keep the sequences ``rows``: an index along the batch (repeats and negative
+        ones allowed), or a truth value for each."""
         with _normal_tensors():
-            rows = rows.to(self.device, torch.int64)
+            rows = rows.to(self.device)
+            rows = rows.nonzero().flatten() if rows.dtype is torch.bool else rows.to(torch.int64)
+            rows = torch.where(rows < 0, rows + self.batch, rows)
             lengths = self.lengths.index_select(0, rows)
             self._take([t.index_select(0, rows) for t in self.buffers])
         self._lengths = lengths

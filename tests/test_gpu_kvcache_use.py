@@ -108,3 +108,14 @@ def test_numbers_beyond_32_bits_are_refused():
             with pytest.raises((ValueError, RuntimeError)):
                 call()
     assert all(torch.equal(a, b) for a, b in zip(before, c.buffers))
+
+
+def test_select_takes_what_indexing_takes():
+    """Truth values and indexes from the end, as transformers' layers do."""
+    dev = _dev()
+    c, k, v = _cache(dev, B=4)
+    want = c.read()[0]
+    c.select(torch.tensor([True, False, True, True]))
+    assert c.batch == 3 and torch.equal(c.read()[0], want[[0, 2, 3]])
+    c.select(torch.tensor([-1, 0], device=dev))
+    assert c.lengths.tolist() == [60, 60] and torch.equal(c.read()[0], want[[3, 0]])
