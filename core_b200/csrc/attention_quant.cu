@@ -794,22 +794,32 @@ Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len) {
   return r;
 }
 
-// The plan of the workspace query serves the call that follows it.
-Plan plan(int bits, int B, int Hkv, long long rows, int max_len) {
+Plan whole_plan(int bits, int B, int Hkv, long long rows, int max_len) {
+  Plan p = make_plan(bits, B, Hkv, rows, max_len);
+  // A warp a row where rows are many for their parts, else a CTA a row: 16384 rows of
+  // 2 parts 171 -> 153 us with the attention itself, 2048 rows of 8 parts 31.2 -> 34.9.
+  p.join_rows = rows * B * Hkv > (long long)sm_count() * 8 * p.n_split;
+  return p;
+}
+
+// The plan of the workspace query serves the call of the same sizes that follows it on
+// this thread, also if the SMs to plan for were changed in between (another thread
+// may): the workspace fits that plan.
+Plan plan(int bits, int B, int Hkv, long long rows, int max_len, bool query) {
   struct Last {
-    long long key[6];
+    long long key[5];
+    int sms;
     Plan plan;
   };
-  static thread_local Last last{{-1, 0, 0, 0, 0, 0}, {}};
-  const long long key[6] = {bits, B, Hkv, rows, max_len, sm_count()};
-  bool same = true;
-  for (int i = 0; i < 6; ++i) same = same && key[i] == last.key[i];
+  static thread_local Last last{{-1, 0, 0, 0, 0}, 0, {}};
+  const long long key[5] = {bits, B, Hkv, rows, max_len};
+  const int sms = sm_count();
+  bool same = !query || sms == last.sms;
+  for (int i = 0; i < 5; ++i) same = same && key[i] == last.key[i];
   if (!same) {
-    last.plan = make_plan(bits, B, Hkv, rows, max_len);
-    // A warp a row where rows are many for their parts, else a CTA a row: 16384 rows of
-    // 2 parts 171 -> 153 us with the attention itself, 2048 rows of 8 parts 31.2 -> 34.9.
-    last.plan.join_rows = rows * B * Hkv > (long long)sm_count() * 8 * last.plan.n_split;
-    for (int i = 0; i < 6; ++i) last.key[i] = key[i];
+    last.plan = whole_plan(bits, B, Hkv, rows, max_len);
+    last.sms = sms;
+    for (int i = 0; i < 5; ++i) last.key[i] = key[i];
   }
   return last.plan;
 }
@@ -862,7 +872,7 @@ extern "C" size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, in
       cache->batch <= 0 || max_length < 0)
     return 0;
   const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
-  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length);
+  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length, true);
   SizerOut z;
   float *a, *b;
   carve_parts(z, pl.n_split, rows * cache->batch * cache->n_kv_heads, &a, &b);
@@ -882,7 +892,7 @@ extern "C" int core_kvq_attention_plan(const core_kvq_t* cache, int32_t n_q_head
     return set_error(CORE_ERR_INVALID_ARG, f + ": max_length outside the cache's capacity");
   const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
   if (rows > INT_MAX / 2) return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
-  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length);
+  const kvq::Plan pl = kvq::whole_plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length);
   out->row_tile = pl.many ? kvq::kManyRows : 8 * pl.nt;
   out->ctas_per_sm = pl.ctas;
   out->parts = pl.n_split;
@@ -943,7 +953,7 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
   p.out = out;
   p.lse = lse;
   p.status = device_status();
-  const kvq::Plan pl = kvq::plan(cache->bits, p.B, p.Hkv, rows, max_length);
+  const kvq::Plan pl = kvq::plan(cache->bits, p.B, p.Hkv, rows, max_length, false);
   p.n_rt = pl.n_rt;
   p.n_split = pl.n_split;
   Carver c(workspace, workspace_bytes);

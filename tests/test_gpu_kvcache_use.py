@@ -119,3 +119,25 @@ def test_select_takes_what_indexing_takes():
     assert c.batch == 3 and torch.equal(c.read()[0], want[[0, 2, 3]])
     c.select(torch.tensor([-1, 0], device=dev))
     assert c.lengths.tolist() == [60, 60] and torch.equal(c.read()[0], want[[3, 0]])
+
+
+def test_attention_after_the_sm_budget_changed():
+    """The workspace that was asked for serves the call of the same sizes, although
+    another thread changed the process-wide SM budget in between."""
+    import ctypes
+    from core_b200 import _lib, ops
+    dev = _dev()
+    c, _, _ = _cache(dev, B=1, n=3000, cap=3072)
+    q = _rows(311, (1, 8, 1, 128), torch.bfloat16).to(dev)
+    want, _ = ops.attention_quantized(q, c, 3000)
+    lib = _lib.load()
+    with ops.sm_budget(8):
+        need = lib.core_kvq_attention_workspace_bytes(c.handle, 8, 1, 3000)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    out, lse = torch.empty(1, 1, 8, 128, dtype=torch.bfloat16, device=dev), torch.empty(1, 8, 1, device=dev)
+    strides = (ctypes.c_int64 * 3)(*q.stride()[:3])
+    rc = lib.core_kvq_attention(c.handle, _lib.CORE_DTYPE_BF16, 8, 1, q.data_ptr(), strides, None, 3000, None, 0, 1,
+                                128 ** -0.5, out.data_ptr(), lse.data_ptr(), ws.data_ptr() if need else None, need,
+                                torch.cuda.current_stream(dev).cuda_stream)
+    assert rc == 0, _lib.last_error()
+    assert (out.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
