@@ -21,6 +21,12 @@ from . import attention, ops
 from .kvcache import QuantizedKV
 
 
+def _room(tokens: int) -> int:
+    """Slots for a layer of ``tokens``: an eighth more, and 256 at least, so that the
+    buffers stay close to their rows and decoding copies them rarely."""
+    return tokens + max(256, tokens // 8)
+
+
 class QuantizedCacheLayer(CacheLayerMixin):
     """One layer: a ``QuantizedKV`` that grows as tokens arrive."""
 
@@ -37,10 +43,12 @@ class QuantizedCacheLayer(CacheLayerMixin):
         if key_states.shape[-1] != ops.HEAD_DIM or value_states.shape != key_states.shape:
             raise ValueError(f"the quantised cache takes keys and values of head_dim {ops.HEAD_DIM}")
         self.dtype, self.device = key_states.dtype, key_states.device
-        B, H = key_states.shape[:2]
-        self.kv = QuantizedKV.empty(B, H, 2 * key_states.shape[2] + 128, bits=self.bits,
-                                    group=self.group, device=self.device)
+        self.kv = self._empty(key_states)
         self.is_initialized = True
+
+    def _empty(self, rows: torch.Tensor) -> QuantizedKV:
+        B, H, n = rows.shape[:3]
+        return QuantizedKV.empty(B, H, _room(n), bits=self.bits, group=self.group, device=rows.device)
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
         if self.kv is None:
@@ -48,7 +56,7 @@ class QuantizedCacheLayer(CacheLayerMixin):
         kv, n = self.kv, key_states.shape[2]
         first = kv.max_length == 0
         if kv.max_length + n > kv.capacity:
-            kv.reserve(2 * (kv.max_length + n))
+            kv.reserve(_room(kv.max_length + n))
         kv.append(key_states, value_states)
         if first:
             return key_states, value_states
@@ -70,12 +78,12 @@ class QuantizedCacheLayer(CacheLayerMixin):
         return self.kv.read(dtype=self.dtype)
 
     def write_rows(self, keys: torch.Tensor, values: torch.Tensor) -> None:
-        """Replace every row (a press stores the ones it kept)."""
+        """Replace every row (a press stores the ones it kept), in buffers of their size."""
         if self.kv is None:
             self.lazy_initialization(keys, values)
-        self.kv.reset()
-        self.kv.reserve(keys.shape[2])
-        self.kv.append(keys, values)
+        kv = self._empty(keys)
+        kv.append(keys, values)
+        self.kv = kv
 
     def get_seq_length(self) -> int:
         return 0 if self.kv is None else self.kv.max_length

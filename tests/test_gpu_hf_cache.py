@@ -168,3 +168,34 @@ def test_prompt_under_inference_mode_decoding_under_no_grad():
         cache.crop(40)
         cache.reset()
     assert torch.equal(torch.cat(got, 1).float(), want)
+
+
+def test_room_follows_the_rows():
+    """A layer holds little more than its rows: after the prompt, as tokens come, and
+    after a press kept a quarter; 4 bits take less than a third of bf16 throughout."""
+    from core_b200.hf_cache import QuantizedCacheLayer
+    dev = _dev()
+    layer = QuantizedCacheLayer(bits=4, group=64)
+    k = torch.randn(1, 2, 16384, 128, device=dev, dtype=torch.bfloat16)
+
+    def check(n):
+        assert layer.get_seq_length() == n
+        row = 2 * 2 * (64 + 8)  # K and V of two heads: codes, scales and zeros
+        assert layer.kv.nbytes <= row * (n + max(256, n // 8) + 127)
+
+    layer.update(k, -k)
+    check(16384)
+    for t in range(2100):
+        layer.update(k[:, :, t:t + 1], -k[:, :, t:t + 1])
+    check(18484)
+    rows = layer.read_rows()
+    assert torch.equal(rows[0][:, :, 16384:], rows[0][:, :, :2100])
+    kept = [r[:, :, ::4].contiguous() for r in rows]
+    layer.write_rows(*kept)
+    check(4621)
+    before = layer.read_rows()
+    with pytest.raises((ValueError, TypeError)):  # a refusal leaves the rows as they were
+        layer.write_rows(kept[0], kept[1].double())
+    assert layer.get_seq_length() == 4621 and torch.equal(layer.read_rows()[0], before[0])
+    layer.update(k[:, :, :300], -k[:, :, :300])
+    check(4921)
