@@ -199,3 +199,102 @@ def test_room_follows_the_rows():
     assert layer.get_seq_length() == 4621 and torch.equal(layer.read_rows()[0], before[0])
     layer.update(k[:, :, :300], -k[:, :, :300])
     check(4921)
+
+
+@pytest.mark.parametrize("bits,group", [(4, 64), (8, 128)])
+def test_a_press_keeps_codes_as_they_are(monkeypatch, bits, group):
+    """The CORE press over a model with this cache: prefill compression and the
+    recompressions while decoding.  Rows read back as bf16 quantise to the codes, scales
+    and zeros that they came from, so the kept rows stay bit for bit."""
+    from core_b200 import attention, ops, press as P
+    from core_b200.hf_cache import quantized_cache
+    from helpers import HOOK_CASE, load_case
+    from test_gpu_kvcache import _decode
+    from transformers import LlamaConfig, LlamaForCausalLM
+    dev = _dev()
+    _, meta = load_case(HOOK_CASE)
+    attention.register()
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(LlamaConfig(
+        vocab_size=97, hidden_size=meta["hidden"], intermediate_size=256, num_hidden_layers=2,
+        num_attention_heads=meta["hq"], num_key_value_heads=meta["hkv"], head_dim=128, max_position_embeddings=4096,
+        attn_implementation="core_b200")).to(dev, torch.bfloat16).eval()
+    press = P.load_core_prefill_decoding_press("tests/golden/core_indexer_hook.pt", device=str(dev),
+                                               compression_ratio=0.5, decoding_compression_interval=4)
+    ids = torch.randint(0, 97, (1, 300), generator=torch.Generator().manual_seed(7)).to(dev)
+    cache = quantized_cache(model.config, bits=bits, group=group)
+    before, events = {}, []  # a layer's rows when the press reads them; what it keeps
+    scorer = press.prefilling_press.base_press
+    read, retain = P.read_cache_layer, scorer.retain_metadata
+
+    def reading(c, layer):
+        before[layer] = _decode(c.layers[layer].kv)
+        return read(c, layer)
+
+    def retaining(layer, keep):
+        events.append((int(layer), keep[0].long().cpu()))
+        return retain(layer, keep)
+
+    monkeypatch.setattr(P, "read_cache_layer", reading)
+    monkeypatch.setattr(scorer, "retain_metadata", retaining)
+    press.reset_cache()
+    press.begin_sequence(290)
+    press.set_token_ids(ids[:, :290])
+    with torch.no_grad(), press(model):
+        model(ids[:, :290], past_key_values=cache, cache_position=torch.arange(290, device=dev))
+        for t in range(290, 300):
+            n = cache.get_seq_length()
+            if events:
+                assert [e[0] for e in events] == [0, 1] and n == 145
+            for layer, keep in events:
+                kv = cache.layers[layer].kv
+                assert kv.max_length == len(keep) and kv.lengths.tolist() == [len(keep)]
+                for got, want in zip(_decode(kv), before[layer]):
+                    assert torch.equal(got[0, :, :len(keep)], want[0][:, keep])
+            events.clear()
+            pid = torch.tensor([[t]], device=dev)
+            press.record_input_tokens(ids[:, t:t + 1], pid)
+            model(ids[:, t:t + 1], past_key_values=cache, position_ids=pid,
+                  cache_position=torch.tensor([n], device=dev))
+    ops.status(dev)
+    assert cache.get_seq_length() == 145 + 2  # two recompressions in ten steps, two tokens since
+
+
+def test_a_press_that_drops_nothing_or_writes_in_place(monkeypatch):
+    """Rows that a press returns as they were keep their codes; what it wrote into them is stored."""
+    from core_b200 import press as P
+    from core_b200.hf_cache import quantized_cache
+    dev = _dev()
+    model = _model(dev, "core_b200")
+    ids = torch.randint(0, 97, (1, 50), generator=torch.Generator().manual_seed(8)).to(dev)
+    before, read = {}, P.read_cache_layer
+
+    def reading(c, layer):
+        before[layer] = [t.clone() for t in c.layers[layer].kv.buffers]
+        return read(c, layer)
+
+    monkeypatch.setattr(P, "read_cache_layer", reading)
+
+    class Nothing(P.BasePress):
+        def compress(self, module, hidden_states, keys, values, attentions, kwargs):
+            return keys, values
+
+    class Halves(P.BasePress):
+        def compress(self, module, hidden_states, keys, values, attentions, kwargs):
+            before["rows"] = keys.clone()
+            keys.mul_(0.5)
+            return keys, values
+
+    for kind in (Nothing, Halves):
+        for mode in (torch.no_grad, torch.inference_mode):
+            cache = quantized_cache(model.config, bits=8, group=128)
+            at = torch.arange(50, device=dev)
+            with mode(), kind()(model):
+                model(ids, past_key_values=cache, cache_position=at)
+            kv = cache.layers[1].kv
+            assert kv.max_length == 50
+            if kind is Halves:
+                rows = before["rows"].float()
+                assert (kv.read()[0].float() - 0.5 * rows).norm() < 0.1 * rows.norm()
+            else:
+                assert all(torch.equal(a[:, :, :50], b[:, :, :50]) for a, b in zip(kv.buffers, before[1]))
