@@ -25,8 +25,8 @@
 //    they become f16 values n s + z (one rounding, 2^-12) in registers.
 //  * A warp owns 32-token tiles (every fourth of its CTA's) with its own ring of
 //    bulk copies, running maxima and sums: nothing waits for another warp until
-//    the CTA's four results are joined.  The maximum is raised only when a score
-//    passes it by 2^7.
+//    the CTA's four results are joined.  Sums are rescaled only when a score
+//    passes the maximum that they were scaled with by 2^7.
 //  * A sequence is cut over CTAs when there are few (batch row, KV head) pairs; a
 //    second kernel, set up while the parts run, joins them.  Which kernel takes a
 //    call and into how many parts is decided by modelled times (below).
@@ -242,10 +242,10 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
   }
 
   float o[8][kNT][4];
-  float m_used[kNT][2], l[kNT][2];
+  float anchor[kNT][2], l[kNT][2];
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
-    m_used[n][0] = m_used[n][1] = -INFINITY;
+    anchor[n][0] = anchor[n][1] = -INFINITY;
     l[n][0] = l[n][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
           }
     }
 
-    // ---- running maxima
+    // ---- running maxima, as the anchors of P
     bool raise = false;
     float mx[kNT][2];
 #pragma unroll
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         mx[n][h] = fmaxf(fmaxf(sc[0][n][h], sc[0][n][h + 2]), fmaxf(sc[1][n][h], sc[1][n][h + 2]));
-        raise |= mx[n][h] - m_used[n][h] > kRaise;
+        raise |= mx[n][h] - anchor[n][h] > kTop;
       }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -420,9 +420,9 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          if (v - m_used[n][h] > kRaise) {
-            const float f = ex2_approx(m_used[n][h] - v);
-            m_used[n][h] = v;
+          if (v - anchor[n][h] > kTop) {
+            const float f = ex2_approx(anchor[n][h] - (v - kLift));
+            anchor[n][h] = v - kLift;
             l[n][h] *= f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -437,8 +437,8 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
     uint32_t pf[2][kNT][2];
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      const float b0 = m_used[n][0] == -INFINITY ? 0.f : m_used[n][0] - kLift;
-      const float b1 = m_used[n][1] == -INFINITY ? 0.f : m_used[n][1] - kLift;
+      const float b0 = anchor[n][0] == -INFINITY ? 0.f : anchor[n][0];
+      const float b1 = anchor[n][1] == -INFINITY ? 0.f : anchor[n][1];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         const float e0 = ex2_approx(sc[mt][n][0] - b0), e1 = ex2_approx(sc[mt][n][1] - b1);
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
       v += __shfl_xor_sync(0xffffffffu, v, 8);
       v += __shfl_xor_sync(0xffffffffu, v, 16);
       if (g == 0) {
-        sm_m[warp][8 * n + 2 * t + h] = m_used[n][h];
+        sm_m[warp][8 * n + 2 * t + h] = anchor[n][h];
         sm_l[warp][8 * n + 2 * t + h] = v;
       }
     }
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kAttnThreads, kCtas) attn_few_kernel(const Att
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) sm_m[w][r] = f[w] * inv;
-    const float lse2 = lt == 0.f ? -INFINITY : m + (log2f(lt) - kLift);
+    const float lse2 = lt == 0.f ? -INFINITY : m + log2f(lt);
     if (row < rows) {
       if (p.n_split > 1) {
         const long long at = ((long long)bh * rows + row) * p.n_split + split;

@@ -10,11 +10,12 @@
 namespace core {
 namespace kvq {
 
-// A running maximum is raised when a score passes it by more than kRaise (in powers of
-// two; compared as a difference, which is exact), and P = 2^(S - maximum + kLift): 2^14
-// at most, which leaves f16 room for what rounding adds to maxima above 2^23, down to
-// 2^-25, 2^-32 of a row's largest.  Without the lift a long tail of weights of 2^-25 was lost.
-constexpr float kRaise = 7.0f, kLift = 7.0f;
+// P = 2^(S - anchor): a row's anchor lies kLift (in powers of two) below its maximum when it
+// was last raised, and is raised when a score passes it by more than kTop (a difference,
+// which is exact).  So P is 2^14 at most, which leaves f16 room for what rounding adds to
+// scores above 2^23, and goes down to 2^-25, 2^-32 of the row's largest.  With the maximum
+// itself as anchor a long tail of weights of 2^-25 was lost.
+constexpr float kLift = 7.0f, kTop = 14.0f;
 
 struct AttnParams {
   const uint8_t* kc;

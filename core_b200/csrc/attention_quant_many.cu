@@ -35,8 +35,8 @@
 //
 // Keys and values are rounded to f16 (2^-11; bf16 would lose three more bits),
 // queries stay exact behind a power of two per row, P is f16 (2^7 at the running
-// maximum, at most 2^14), sums and statistics are f32.  The maximum of a row is
-// raised, and O_x rescaled, only when a score passes it by 2^7.
+// maximum, at most 2^14), sums and statistics are f32.  O_x is rescaled only when a score
+// passes the maximum that it was scaled with by 2^7.
 #include <cuda_bf16.h>
 
 #include "attention_quant.cuh"
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
       const uint32_t tS = lanes + kColS, tP = lanes + kColP + 64u * x, tO = lanes + kColO + 128u * x;
       const unsigned long long sc2 = f2_pack(sc, sc);
-      float m_used = -INFINITY, l = 0.f;
+      float anchor = -INFINITY, l = 0.f;
       bool ok = true;
       // a tile's mask is asked for while the tile before it is worked on
       uint32_t seen[4] = {1u, 1u, 1u, 1u};
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
           for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], v[e + 2 * c], v[e + 2 * c + 1]);
         }
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-        const bool raise = mt - m_used > kRaise;
+        const bool raise = mt - anchor > kTop;
         // O_x holds every earlier tile, and P_x may be written again, once the last
         // P V has landed
         auto last_pv = [&]() -> bool {
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
           return __all_sync(0xffffffffu, got);
         };
         if (__any_sync(0xffffffffu, raise)) {
-          const float f = raise ? ex2_approx(m_used - mt) : 1.0f;
+          const float f = raise ? ex2_approx(anchor - (mt - kLift)) : 1.0f;
           if (j > 0) {
             if (!(ok = last_pv())) break;
             l *= f;
@@ -552,9 +552,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
               tmem_st16(tO + 16u * c, o);
             }
           }
-          if (raise) m_used = mt;
+          if (raise) anchor = mt - kLift;
         }
-        const float neg = m_used == -INFINITY ? 0.f : kLift - m_used;
+        const float neg = anchor == -INFINITY ? 0.f : -anchor;
         const unsigned long long neg2 = f2_pack(neg, neg);
         unsigned long long acc = 0ull;
 #pragma unroll
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       if (ok) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that saw no token: output 0, LSE -inf
-        const float lse2 = l == 0.f ? -INFINITY : m_used + (log2f(l) - kLift);
+        const float lse2 = l == 0.f ? -INFINITY : anchor + log2f(l);
         const long long part = ((long long)bh * rows + row) * p.n_split + split;
         const int Hq = p.Hkv * p.G;
         float* of = p.n_split > 1 ? p.part_o + part * kD : nullptr;
