@@ -5,24 +5,27 @@
 //
 // What bounds it: the packed cache is read once, 16 bits + 4 (128 / group) bytes a
 // row of K or V; beside that, every code has to be turned into a matrix operand.
-// In 8 bits the bytes bind: 8 x 32768 tokens of 8 heads 94 us, 6.0 TB/s.  In 4 bits
-// the instructions do: 680 a tile of 32 tokens and warp, issued at 61% of the peak
-// by 16 warps an SM, 67-70 us (4.3-4.9 TB/s); one sequence of 131072 tokens
-// takes 41 us, 24 of them at the rate of memory.  Half of the instructions go
-// through the half-rate integer pipe that masks and pairs the nibbles.
+// In 8 bits the bytes bind: 8 x 32768 tokens of 8 heads 91-101 us by the group, 6.0-6.2
+// TB/s; one sequence of 131072 tokens 49 us, 5.8 TB/s.  In 4 bits neither the bytes
+// (8 x 32768 tokens 67-70 us, 4.3-4.9 TB/s; 131072 tokens 41 us, 24 of them at the
+// rate of memory) nor the issue slots (62% and 58% used) are full: the 670
+// instructions of a tile of 32 tokens and warp depend on one another (K's codes,
+// products, maximum, exponent, transpose, V's codes), and the 16 or 12 warps that an SM
+// holds do not cover all of it.  Half of the instructions go through the half-rate
+// integer pipe that masks and pairs the nibbles (55% busy).
 //
 //  * The codes are the A operand (16 tokens, or 16 channels, a tile) and the
 //    query rows the 8 columns of B (up to three such tiles a CTA), so that a GQA
-//    group of up to 8 rows wastes little; S^T comes out with a token per row and goes back in as the B
-//    operand of P V through movmatrix, without leaving the registers.
+//    group of up to 8 rows wastes little; S^T comes out with a token per row and goes
+//    back in as the B operand of P V through movmatrix, without leaving the registers.
 //  * K's codes enter as exact integers: a nibble masked out of its word is the
 //    f16 subnormal n 2^-24 (or 16 n 2^-24; q then carries the 1/16).  A group's
 //    products are multiplied by its scale in f32, and the zeros come in through
 //    one more product, z times the row's sum of q over the group (as two f16
 //    terms), so that S has no rounding but f32's.  q is scaled by a power of two
-//    to f16's range per row; bf16 and f16 queries stay exact.
+//    to f16's range per row; its elements stay exact down to 2^-18 of the row's largest.
 //  * V's codes are spread over tokens in the scale that multiplies them, so
-//    they become f16 values n s + z (one rounding, 2^-12) in registers.
+//    they become f16 values n s + z (one rounding, 2^-11) in registers.
 //  * A warp owns 32-token tiles (every fourth of its CTA's) with its own ring of
 //    bulk copies, running maxima and sums: nothing waits for another warp until
 //    the CTA's four results are joined.  Sums are rescaled only when a score

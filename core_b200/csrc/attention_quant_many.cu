@@ -27,16 +27,18 @@
 // to ask for them (475 to 590 us for 2048 queries over 16384 tokens; 492-522 now,
 // in every format).
 //
-// What bounds it now: 512 queries (2048 rows a head) over 16384 tokens take 170 us,
-// 800 TFLOP/s, and 2048 queries 492 us, 1.1 PFLOP/s of the measured 1.65.  A pair
-// of tiles takes about 3500 cycles, of which the MMAs need 2048: Q K^T reads 128
-// bytes of shared memory a cycle, all there are, and shares them with the tiles'
-// writing; the rest is the way of S from tensor core to registers and back.
+// What bounds it now: 512 queries (2048 rows a head) over 16384 tokens take 149 us,
+// join included, 910 TFLOP/s, and 2048 queries 486 us, 1.06 PFLOP/s of the measured
+// 1.65.  A pair of tiles takes about 3500 cycles, of which the MMAs need 2048: Q K^T
+// reads 128 bytes of shared memory a cycle, all there are, and shares them with the
+// tiles' writing; the rest is the way of S from tensor core to registers and back.  The
+// softmax spills (116-120 bytes of stores in the six builds: 128 scores of a row and
+// their state against 168 registers).
 //
-// Keys and values are rounded to f16 (2^-11; bf16 would lose three more bits),
-// queries stay exact behind a power of two per row, P is f16 (2^7 at the running
-// maximum, at most 2^14), sums and statistics are f32.  O_x is rescaled only when a score
-// passes the maximum that it was scaled with by 2^7.
+// Keys and values are rounded to f16 (2^-11; bf16 would lose three more bits), queries
+// stay exact, behind a power of two per row, down to 2^-21 of the row's largest, P is f16
+// (2^7 at the running maximum, at most 2^14), sums and statistics are f32.  O_x is
+// rescaled only when a score passes the maximum that it was scaled with by 2^7.
 #include <cuda_bf16.h>
 
 #include "attention_quant.cuh"

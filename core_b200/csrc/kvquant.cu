@@ -14,10 +14,11 @@
 // flight, group extrema come from shuffles (16-bit types: least and minus greatest
 // in one register), the codes from shifted sums of the floats' bit patterns, the
 // clamp only for groups that need it.  It is bound by the instructions it issues
-// (460 for 16 channels of K and V a lane, 80% of the issue slots) close to the
-// memory's time: 16384 tokens of 8 heads in bf16 17.7 us (4.8 TB/s), 8 x 32768 242
-// us (5.8 TB/s).  Reading back is bound by memory: 8 x 32768 tokens 214 us (6.6
-// TB/s), 16384 tokens 16 us.  Blocks of 128 threads, twelve an SM, gave 5% over
+// (460 for 16 channels of K and V a lane, 84% of the issue slots) close to the
+// memory's time: 16384 tokens of 8 heads in bf16 16.3 us (5.3 TB/s), 8 x 32768 242
+// us (5.8 TB/s).  From f32, eight blocks an SM, it is bound by memory: 16384 tokens 24.4
+// us (6.3 TB/s).  So is reading back: 8 x 32768 tokens 213 us (6.6 TB/s), 16384 tokens
+// 15.0 us.  Blocks of 128 threads, twelve an SM, gave 5% over
 // blocks of 256.
 #include <cuda_bf16.h>
 

@@ -313,6 +313,12 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     ``key_mask`` (B, n >= max_length) bool or uint8: False hides a token.
     Returns (out (B, Lq, Hq, 128) in q's dtype, lse (B, Hq, Lq) f32); a row that
     sees no token gives 0 and -inf.
+
+    Statistics, sums and the LSE are f32, the weights and the cached values f16.  Up to
+    32 query rows a KV head (Lq times the heads that share it) scores are exact to f32;
+    with more, the faster kernel for the sizes may round the keys to f16 as well, which
+    moves scores and LSE by up to 2^-11 softmax_scale sum |q||k|
+    (:func:`attention_quantized_plan` tells).  No gradient is recorded.
     """
     if q.get_device() != cache.index:
         raise _wrong_device(q, "q")

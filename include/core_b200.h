@@ -448,10 +448,12 @@ int core_attention_prefill(const core_dims_t* dims, const void* q, const int64_t
  *
  * A row is one token of one KV head, 128 channels.  Each group of `group`
  * neighbouring channels has an f16 scale s and zero z; a code n stands for
- * n s + z:  lo, hi = least and greatest value of the group within +-61440,
- * z = f16(lo), s = f16((hi - lo) / N), n = rint((x - z) / s) kept in 0..N,
- * N = 15 or 255 (each step rounded once in f32).  Values beyond +-61440
- * saturate; a group that holds a NaN reads back as NaN.
+ * n s + z.  With lo, hi = least and greatest value of the group within +-61440,
+ * N = 15 or 255 and c = f32(1 / N):
+ *   z = f16(lo)   s = f16((hi - lo) c)   i = f32(1 / s), 0 where s = 0
+ *   n = rint((x - z) i) kept in 0..N
+ * where every difference and product is rounded to f32 by itself.  Values beyond
+ * +-61440 saturate; a group that holds a NaN reads back as NaN.
  *   codes : (B, Hkv, capacity, 16 * bits) bytes
  *   meta  : (B, Hkv, capacity, 128 / group, 2) f16, (s, z)
  * capacity is a multiple of 128; all four buffers are 16-byte aligned and may
@@ -506,8 +508,16 @@ int core_kvq_dequantize(const core_kvq_t* cache, int32_t dtype, int32_t n_rows, 
  *              0: all of them
  *   out      : (B, n_queries, n_q_heads, 128) in q's dtype
  *   lse      : (B, n_q_heads, n_queries) f32, natural log
- * A row that sees no token gives 0 and -inf.  Hidden tokens count for nothing
- * whatever their bytes hold. */
+ * A row that sees no token gives 0 and -inf.  A token that key_mask hides, or at or
+ * past the sequence's length, counts for nothing whatever its bytes hold.  One that
+ * only the causal limit hides from some queries of the call has to be finite: its
+ * value meets their weight of 0, and a NaN there can reach them.
+ * Precision: sums, statistics and the LSE are f32; P and the values n s + z are
+ * rounded to f16 (2^-11).  Up to 32 query rows a KV head (queries x heads that share
+ * it) scores are f32 sums of exact products.  Above that the plan may choose the
+ * kernel on tcgen05, by modelled time, which rounds n s + z of the keys to f16 as well
+ * (scores and LSE off by at most 2^-11 softmax_scale sum |q||k|): core_kvq_attention_plan
+ * tells for given sizes.  Queries keep f16's eleven bits down to 2^-18 of their row's largest. */
 size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries,
                                           int32_t max_length);
 
