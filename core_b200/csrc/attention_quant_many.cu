@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
   auto bar_s_taken = [&](int x) { return bar + 96 + 8u * x; };  // they are in registers
   auto bar_p_full = [&](int x) { return bar + 112 + 8u * x; };
   auto bar_pv = [&](int x) { return bar + 128 + 8u * x; };
+  auto bar_last = [&](int w) { return bar + 144 + 8u * w; };  // an MMA warp that gives up: its products are done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + ManySmem::kBar + 400);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + ManySmem::kBar + 408);
 
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       mbar_init(bar_s_taken(i), 4);
       mbar_init(bar_p_full(i), 4);
       mbar_init(bar_pv(i), 1);
+      mbar_init(bar_last(i), 1);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -367,9 +369,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
       return got;
     };
     bool ok = n > 0;
+    const bool leader = elect_one();
     if (warp == 16) {
       constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kManyTok >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-      const bool leader = elect_one();
       for (int j = 0; j < n && ok; ++j) {
         if (!(ok = all(bar_k_full(j & 1), (uint32_t)(j >> 1) & 1u, 1431))) break;
         const uint64_t kd = sdesc_kmajor(sK + (uint32_t)(j & 1) * kTile);
@@ -394,7 +396,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
     } else if (warp == 17) {
       constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24) |
                                  (1u << 16);  // B (the V tile) MN-major
-      const bool leader = elect_one();
       for (int j = 0; j < n && ok; ++j) {
         if (!(ok = all(bar_v_full(j & 1), (uint32_t)(j >> 1) & 1u, 1434))) break;
         const uint64_t vd = sdesc_sw128(sV + (uint32_t)(j & 1) * kTile, kAtom, 1024u);
@@ -410,6 +411,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_many_kernel(const AttnPa
           }
           __syncwarp();
         }
+      }
+    }
+    if (!ok && n > 0) {  // given up: no product may be in flight when TMEM is freed
+      if (leader) mma_commit(bar_last(warp - 16));
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(bar_last(warp - 16), 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
       }
     }
   } else if (warp >= 8) {
