@@ -97,7 +97,7 @@ def test_numbers_beyond_32_bits_are_refused():
     from core_b200 import ops
     dev = _dev()
     c, k, v = _cache(dev)
-    before = [t.clone() for t in c.buffers]
+    before = [t.view(torch.uint8).clone() for t in c.buffers]
     q = _rows(310, (2, 4, 1, 128), torch.bfloat16).to(dev)
     at = torch.full((2,), 60, dtype=torch.int32, device=dev)
     for far in (2 ** 32, 2 ** 32 + 3, -2 ** 32, 2 ** 31):
@@ -107,7 +107,7 @@ def test_numbers_beyond_32_bits_are_refused():
                      lambda: ops.attention_quantized_plan(c, 4, 1, far)):
             with pytest.raises((ValueError, RuntimeError)):
                 call()
-    assert all(torch.equal(a, b) for a, b in zip(before, c.buffers))
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, c.buffers))
 
 
 def test_select_takes_what_indexing_takes():
