@@ -91,6 +91,7 @@ class CoreKvqPlan(ctypes.Structure):
         ("parts", ctypes.c_int32),
         ("join_rows", ctypes.c_int32),
         ("f16_keys", ctypes.c_int32),
+        ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -149,7 +150,7 @@ SIGNATURES = {
     "core_kvq_quantize": (ctypes.c_int, [_Q, _I, _P, _P, _P, _P, _I, _I, _P, _P, _I, _P, _P]),
     "core_kvq_dequantize": (ctypes.c_int, [_Q, _I, _I, _P, _P, _I, _P, _P, _P]),
     "core_kvq_attention_workspace_bytes": (_S, [_Q, _I, _I, _I]),
-    "core_kvq_attention_plan": (ctypes.c_int, [_Q, _I, _I, _I, ctypes.POINTER(CoreKvqPlan)]),
+    "core_kvq_attention_plan": (ctypes.c_int, [_Q, _I, _I, _I, _I, ctypes.POINTER(CoreKvqPlan)]),
     "core_kvq_attention": (ctypes.c_int, [_Q, _I, _I, _I, _P, _P, _P, _I, _P, ctypes.c_int64, _I,
                                           _F, _P, _P, _P, _S, _P]),
     "core_compress_layer_workspace_bytes": (_S, [_D, _I, _I]),

@@ -751,7 +751,7 @@ struct Plan {
 // Which kernel takes the call, and into how many parts it cuts the sequences.
 // Tried are the counts that fill the SMs once, twice, .. , each lowered to the
 // least that gives its parts as many tiles.
-Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len) {
+Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len, bool exact) {
   const long long heads = (long long)B * Hkv, sms = sm_count();
   auto least = [](int tiles, int step, long long n) {  // same tiles a part (in `step`s), fewest parts
     const long long most = (tiles + step - 1) / step;
@@ -782,8 +782,8 @@ Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len) {
       }
     }
   }
-  // Up to 32 rows stay with the kernel that keeps the keys exact.
-  if (rows <= 32) return r;
+  // Up to 32 rows stay with the kernel that keeps the keys exact, more where that is asked for.
+  if (rows <= 32 || exact) return r;
   const int many_rt = (int)((rows + kManyRows - 1) / kManyRows), many_tiles = (max_len + kManyTok - 1) / kManyTok;
   const long long many_units = heads * many_rt;
   for (int k = 0; k <= 6; ++k) {
@@ -797,8 +797,8 @@ Plan make_plan(int bits, int B, int Hkv, long long rows, int max_len) {
   return r;
 }
 
-Plan whole_plan(int bits, int B, int Hkv, long long rows, int max_len) {
-  Plan p = make_plan(bits, B, Hkv, rows, max_len);
+Plan whole_plan(int bits, int B, int Hkv, long long rows, int max_len, bool exact) {
+  Plan p = make_plan(bits, B, Hkv, rows, max_len, exact);
   // A warp a row where rows are many for their parts, else a CTA a row: 16384 rows of
   // 2 parts 171 -> 153 us with the attention itself, 2048 rows of 8 parts 31.2 -> 34.9.
   p.join_rows = rows * B * Hkv > (long long)sm_count() * 8 * p.n_split;
@@ -808,21 +808,21 @@ Plan whole_plan(int bits, int B, int Hkv, long long rows, int max_len) {
 // The plan of the workspace query serves the call of the same sizes that follows it on
 // this thread, also if the SMs to plan for were changed in between (another thread
 // may): the workspace fits that plan.
-Plan plan(int bits, int B, int Hkv, long long rows, int max_len, bool query) {
+Plan plan(int bits, int B, int Hkv, long long rows, int max_len, bool exact, bool query) {
   struct Last {
-    long long key[5];
+    long long key[6];
     int sms;
     Plan plan;
   };
-  static thread_local Last last{{-1, 0, 0, 0, 0}, 0, {}};
-  const long long key[5] = {bits, B, Hkv, rows, max_len};
+  static thread_local Last last{{-1, 0, 0, 0, 0, 0}, 0, {}};
+  const long long key[6] = {bits, B, Hkv, rows, max_len, exact};
   const int sms = sm_count();
   bool same = !query || sms == last.sms;
-  for (int i = 0; i < 5; ++i) same = same && key[i] == last.key[i];
+  for (int i = 0; i < 6; ++i) same = same && key[i] == last.key[i];
   if (!same) {
-    last.plan = whole_plan(bits, B, Hkv, rows, max_len);
+    last.plan = whole_plan(bits, B, Hkv, rows, max_len, exact);
     last.sms = sms;
-    for (int i = 0; i < 5; ++i) last.key[i] = key[i];
+    for (int i = 0; i < 6; ++i) last.key[i] = key[i];
   }
   return last.plan;
 }
@@ -875,7 +875,7 @@ extern "C" size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, in
       cache->batch <= 0 || max_length < 0)
     return 0;
   const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
-  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length, true);
+  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length, false, true);
   SizerOut z;
   float *a, *b;
   carve_parts(z, pl.n_split, rows * cache->batch * cache->n_kv_heads, &a, &b);
@@ -883,7 +883,7 @@ extern "C" size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, in
 }
 
 extern "C" int core_kvq_attention_plan(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries,
-                                       int32_t max_length, core_kvq_plan_t* out) {
+                                       int32_t max_length, int32_t causal, core_kvq_plan_t* out) {
   const char* fn = "core_kvq_attention_plan";
   int rc = check_kvq(cache, fn);
   if (rc != CORE_OK) return rc;
@@ -895,12 +895,17 @@ extern "C" int core_kvq_attention_plan(const core_kvq_t* cache, int32_t n_q_head
     return set_error(CORE_ERR_INVALID_ARG, f + ": max_length outside the cache's capacity");
   const long long rows = (long long)(n_q_heads / cache->n_kv_heads) * n_queries;
   if (rows > INT_MAX / 2) return set_error(CORE_ERR_UNSUPPORTED, f + ": too many query rows");
-  const kvq::Plan pl = kvq::whole_plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length);
+  const kvq::Plan pl = kvq::plan(cache->bits, cache->batch, cache->n_kv_heads, rows, max_length,
+                                 (causal & CORE_KVQ_EXACT_KEYS) != 0, true);
   out->row_tile = pl.many ? kvq::kManyRows : 8 * pl.nt;
   out->ctas_per_sm = pl.ctas;
   out->parts = pl.n_split;
   out->join_rows = pl.n_split > 1 && pl.join_rows;
   out->f16_keys = pl.many;
+  SizerOut z;
+  float *a, *b;
+  carve_parts(z, pl.n_split, rows * cache->batch * cache->n_kv_heads, &a, &b);
+  out->workspace_bytes = z.used;
   return CORE_OK;
 }
 
@@ -950,13 +955,14 @@ extern "C" int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_
   p.Lq = n_queries;
   p.cap = cache->capacity;
   p.max_len = max_length;
-  p.causal = causal != 0;
+  p.causal = (causal & ~CORE_KVQ_EXACT_KEYS) != 0;
   p.f16 = dtype == CORE_DTYPE_F16;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.out = out;
   p.lse = lse;
   p.status = device_status();
-  const kvq::Plan pl = kvq::plan(cache->bits, p.B, p.Hkv, rows, max_length, false);
+  const kvq::Plan pl = kvq::plan(cache->bits, p.B, p.Hkv, rows, max_length,
+                                 (causal & CORE_KVQ_EXACT_KEYS) != 0, false);
   p.n_rt = pl.n_rt;
   p.n_split = pl.n_split;
   Carver c(workspace, workspace_bytes);

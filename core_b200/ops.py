@@ -167,6 +167,7 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
 _KVQ_DTYPES = _READOUT_DTYPES
 _I64X3 = ctypes.c_int64 * 3
 _KVQ_SCALE = HEAD_DIM ** -0.5
+_KVQ_EXACT_KEYS = 0x100  # CORE_KVQ_EXACT_KEYS
 
 # One token is written, read or attended to in a few microseconds: these wrappers
 # check in as few calls as they can.
@@ -302,7 +303,8 @@ def kv_dequantize(cache, *, start=0, count: int | None = None, index: torch.Tens
 
 def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | None = None,
                         key_mask: torch.Tensor | None = None, softmax_scale: float | None = None,
-                        causal: bool = True, out: torch.Tensor | None = None):
+                        causal: bool = True, exact_keys: bool = False,
+                        out: torch.Tensor | None = None):
     """Attention of q over a quantised cache, read as codes.
 
     q: (B, Hq, Lq, 128), bf16 or f16, any strides; Hq a multiple of the cache's
@@ -318,14 +320,16 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     32 query rows a KV head (Lq times the heads that share it) scores are exact to f32;
     with more, the faster kernel for the sizes may round the keys to f16 as well, which
     moves scores and LSE by up to 2^-11 softmax_scale sum |q||k|
-    (:func:`attention_quantized_plan` tells).  No gradient is recorded.
+    (:func:`attention_quantized_plan` tells); ``exact_keys`` rules that kernel out.
+    No gradient is recorded.
     """
     if q.get_device() != cache.index:
         raise _wrong_device(q, "q")
     if torch._C._cuda_getDevice() != cache.index:
         with torch.cuda.device(cache.index):
             return attention_quantized(q, cache, lengths, max_length=max_length, key_mask=key_mask,
-                                       softmax_scale=softmax_scale, causal=causal, out=out)
+                                       softmax_scale=softmax_scale, causal=causal, exact_keys=exact_keys,
+                                       out=out)
     dtype = q.dtype
     code = _ATTN_DTYPES.get(dtype)
     if code is None:
@@ -360,10 +364,15 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     if Lq == 0:
         return out, lse
     lib = _lib.load()
-    need = lib.core_kvq_attention_workspace_bytes(cache.handle, Hq, Lq, n)
+    mode = 1 if causal else 0
+    if exact_keys:
+        mode |= _KVQ_EXACT_KEYS
+        need = attention_quantized_plan(cache, Hq, Lq, n, exact_keys=True)["workspace_bytes"]
+    else:
+        need = lib.core_kvq_attention_workspace_bytes(cache.handle, Hq, Lq, n)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     rc = lib.core_kvq_attention(
-        cache.handle, code, Hq, Lq, q.data_ptr(), strides, at, n, mask, mask_stride, causal,
+        cache.handle, code, Hq, Lq, q.data_ptr(), strides, at, n, mask, mask_stride, mode,
         _KVQ_SCALE if softmax_scale is None else softmax_scale, out.data_ptr(), lse.data_ptr(),
         None if ws is None else ws.data_ptr(), need, _raw_stream(cache.index))
     if rc:
@@ -371,15 +380,17 @@ def attention_quantized(q: torch.Tensor, cache, lengths, *, max_length: int | No
     return out, lse
 
 
-def attention_quantized_plan(cache, n_q_heads: int, n_queries: int, max_length: int) -> dict:
+def attention_quantized_plan(cache, n_q_heads: int, n_queries: int, max_length: int, *,
+                             exact_keys: bool = False) -> dict:
     """How :func:`attention_quantized` carries out a call of these sizes: ``row_tile``
     (query rows of a KV head a CTA takes: 8, 16, 24, or 256 on tcgen05), ``ctas_per_sm``,
     ``parts`` (CTAs a sequence is cut over), ``join_rows`` (parts joined by a warp a
-    row) and ``f16_keys`` (keys rounded to f16; otherwise scores are exact to f32)."""
+    row), ``f16_keys`` (keys rounded to f16; otherwise scores are exact to f32) and
+    ``workspace_bytes``."""
     plan = _lib.CoreKvqPlan()
     check(_lib.load().core_kvq_attention_plan(
         cache.handle, _int32(n_q_heads, "n_q_heads"), _int32(n_queries, "n_queries"),
-        _int32(max_length, "max_length"), ctypes.byref(plan)))
+        _int32(max_length, "max_length"), _KVQ_EXACT_KEYS if exact_keys else 0, ctypes.byref(plan)))
     return {name: bool(getattr(plan, name)) if name in ("join_rows", "f16_keys") else getattr(plan, name)
             for name, _ in plan._fields_}
 

@@ -505,7 +505,7 @@ int core_kvq_dequantize(const core_kvq_t* cache, int32_t dtype, int32_t n_rows, 
  *              for all); one outside is clamped and recorded (site 1421)
  *   key_mask : optional (B, mask_stride) bytes, 0 hides a token
  *   causal   : query i sees the tokens before lengths[b] - n_queries + i + 1;
- *              0: all of them
+ *              0: all of them.  CORE_KVQ_EXACT_KEYS may be or-ed to it (below)
  *   out      : (B, n_queries, n_q_heads, 128) in q's dtype
  *   lse      : (B, n_q_heads, n_queries) f32, natural log
  * A row that sees no token gives 0 and -inf.  A token that key_mask hides, or at or
@@ -517,7 +517,10 @@ int core_kvq_dequantize(const core_kvq_t* cache, int32_t dtype, int32_t n_rows, 
  * it) scores are f32 sums of exact products.  Above that the plan may choose the
  * kernel on tcgen05, by modelled time, which rounds n s + z of the keys to f16 as well
  * (scores and LSE off by at most 2^-11 softmax_scale sum |q||k|): core_kvq_attention_plan
- * tells for given sizes.  Queries keep f16's eleven bits down to 2^-18 of their row's largest. */
+ * tells for given sizes, and causal | CORE_KVQ_EXACT_KEYS keeps a call with the kernels
+ * that do not (its workspace: the plan's).  Queries are exact down to 2^-18 of their
+ * row's largest element. */
+#define CORE_KVQ_EXACT_KEYS 0x100
 size_t core_kvq_attention_workspace_bytes(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries,
                                           int32_t max_length);
 
@@ -528,9 +531,10 @@ typedef struct core_kvq_plan {
   int32_t parts;       /* CTAs that a sequence is cut over */
   int32_t join_rows;   /* 1: the parts are joined by a warp a row, 0: by a CTA a row, or not cut */
   int32_t f16_keys;    /* 1: n s + z of the keys is rounded to f16, 0: scores are exact to f32 */
+  size_t workspace_bytes;
 } core_kvq_plan_t;
 int core_kvq_attention_plan(const core_kvq_t* cache, int32_t n_q_heads, int32_t n_queries, int32_t max_length,
-                            core_kvq_plan_t* plan);
+                            int32_t causal, core_kvq_plan_t* plan);
 int core_kvq_attention(const core_kvq_t* cache, int32_t dtype, int32_t n_q_heads, int32_t n_queries,
                        const void* q, const int64_t* q_strides, const int32_t* lengths,
                        int32_t max_length, const uint8_t* key_mask, int64_t mask_stride, int32_t causal,

@@ -51,14 +51,14 @@ def _reference(q, cache, lengths, mask, causal, scale):
     return out, lse, bound, vmax
 
 
-def _check_plan(q, cache, lengths, plan, *, mask=None, causal=True, scale=128 ** -0.5):
+def _check_plan(q, cache, lengths, plan, *, mask=None, causal=True, scale=128 ** -0.5, exact_keys=False):
     """``plan``: what ops.attention_quantized_plan has to say of the call."""
     from core_b200 import ops
-    got = ops.attention_quantized_plan(cache, q.shape[1], q.shape[2], max(lengths))
+    got = ops.attention_quantized_plan(cache, q.shape[1], q.shape[2], max(lengths), exact_keys=exact_keys)
     assert {k: got[k] > 1 if k == "parts" else got[k] for k in plan} == plan, got
     at = torch.tensor(lengths, dtype=torch.int32, device=q.device)
     out, lse = ops.attention_quantized(q, cache, at, max_length=max(lengths), key_mask=mask, causal=causal,
-                                       softmax_scale=scale)
+                                       softmax_scale=scale, exact_keys=exact_keys)
     ops.status(q.device)
     want, wl, bound, vmax = _reference(q, cache, lengths, mask, causal, scale)
     ds = bound * (2.0 ** -20 + (2.0 ** -11 if got["f16_keys"] else 0.0))
@@ -142,6 +142,20 @@ def test_few_rows_tiles_and_joins(bits, group, heads, groups, queries, length, p
     _check_plan(q, c, [length], plan)
     mask = torch.rand(1, length, generator=torch.Generator().manual_seed(223)).to(dev) > 0.3
     _check_plan(q.half(), c, [length], plan, mask=mask)
+
+
+@pytest.mark.parametrize("bits,group", [(4, 64), (8, 32)])
+def test_exact_keys_rules_the_rounding_out(bits, group):
+    """Sizes that go to tcgen05 by themselves: with exact_keys the scores, and so the LSE,
+    are as exact as a few rows', parts and workspace included."""
+    dev = _dev()
+    for batch, heads, groups, queries, length in ((1, 4, 5, 133, 2900), (4, 8, 1, 381, 100)):
+        lengths = [length - 13 * b for b in range(batch)]
+        c = _filled(230, batch, heads, -(-length // 128) * 128, bits, group, dev, lengths)
+        q = _rows(232, (batch, heads * groups, queries, 128), DT["f16"], 2.0).to(dev)
+        _check_plan(q, c, lengths, MANY)
+        for causal in (True, False):
+            _check_plan(q, c, lengths, dict(f16_keys=False), causal=causal, exact_keys=True)
 
 
 @pytest.mark.parametrize("bits", (4, 8))

@@ -88,9 +88,9 @@ def test_attention_plan_on_host():
 
     from core_b200 import ops
 
-    def plan(hq, nq, n, heads=8, cap=1 << 20, bits=4):
+    def plan(hq, nq, n, heads=8, cap=1 << 20, bits=4, **kw):
         kvq = _lib.CoreKvq(256, 256, 256, 256, 1, heads, cap, bits, 64)
-        return ops.attention_quantized_plan(types.SimpleNamespace(handle=ctypes.byref(kvq)), hq, nq, n)
+        return ops.attention_quantized_plan(types.SimpleNamespace(handle=ctypes.byref(kvq)), hq, nq, n, **kw)
 
     for nq in (1, 2, 3, 4, 8):
         p = plan(32, nq, 131072)
@@ -99,9 +99,13 @@ def test_attention_plan_on_host():
     assert plan(8, 1, 0)["parts"] == 1
     p = plan(32, 2048, 16384)
     assert p["f16_keys"] and p["row_tile"] == 256
+    p = plan(32, 2048, 16384, exact_keys=True)
+    assert not p["f16_keys"] and p["row_tile"] < 256
+    one = plan(8, 1, 131072, heads=1)
+    assert one["workspace_bytes"] >= 8 * one["parts"] * 129 * 4
     for bad in (lambda: plan(12, 1, 5), lambda: plan(8, 0, 5), lambda: plan(8, 1, -1), lambda: plan(8, 1, 129, cap=128),
                 lambda: plan(8, 1, 5, bits=3)):
         with pytest.raises(RuntimeError):
             bad()
     assert _lib.load().core_kvq_attention_plan(ctypes.byref(_lib.CoreKvq(256, 256, 256, 256, 1, 8, 128, 4, 64)),
-                                               8, 1, 5, None) == -1
+                                               8, 1, 5, 0, None) == -1
